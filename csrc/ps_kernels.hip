@@ -58,6 +58,8 @@
 
 #include <rocprim/rocprim.hpp>
 
+#include "ops.h"
+
 #define WAVE 64
 #define CHECK_DEV(x) TORCH_CHECK((x).is_cuda(), #x " must be a device tensor")
 #define CHECK_CONT(x) TORCH_CHECK((x).is_contiguous(), #x " must be contiguous")
@@ -2335,4 +2337,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("lr_step", &lr_step, "K9 sparse logistic step",
         py::arg("indptr"), py::arg("feat_slots"), py::arg("x_vals"),
         py::arg("labels"), py::arg("weights"), py::arg("reuse_tag") = 0);
+  m.def("cache_write", &cache_write, "8-bit row records: quantise and write",
+        py::arg("cache"), py::arg("values"), py::arg("slots"),
+        py::arg("fmt"), py::arg("unique"));
+  m.def("cache_read", &cache_read, "8-bit row records: read back",
+        py::arg("cache"), py::arg("dim"), py::arg("slots"), py::arg("fmt"),
+        py::arg("dtype"));
 }

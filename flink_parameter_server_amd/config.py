@@ -44,7 +44,9 @@ class PSConfig:
     # than `staleness` rounds ahead of the slowest worker.
     staleness: Optional[int] = None
 
-    # Wire dtype for pull answers / push deltas ("f32" or "bf16").
+    # Wire dtype for pull answers / push deltas: "f32", "bf16", or 8-bit
+    # row records with one f32 scale a row, "int8" (steps of the row's
+    # largest magnitude / 127) or "fp8" (e4m3; ops.cache_write).
     # Tables always keep f32 master values.
     wire_dtype: str = "f32"
 
@@ -87,7 +89,7 @@ class PSConfig:
             raise ValueError("n_workers and n_shards must be >= 1")
         if self.partitioner not in ("mod", "range"):
             raise ValueError(f"unknown partitioner {self.partitioner!r}")
-        if self.wire_dtype not in ("f32", "bf16"):
+        if self.wire_dtype not in ("f32", "bf16", "int8", "fp8"):
             raise ValueError(f"unknown wire_dtype {self.wire_dtype!r}")
         if self.feedback not in ("fresh", "merged", "pipelined"):
             raise ValueError(f"unknown feedback {self.feedback!r}")

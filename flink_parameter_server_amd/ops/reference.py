@@ -21,7 +21,7 @@ cites are file/symbol level):
 """
 from __future__ import annotations
 
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 
@@ -314,3 +314,82 @@ def sgns_step(vecs: torch.Tensor, center_slots: torch.Tensor,
     deltas.index_add_(0, center_slots, g * u)
     deltas.index_add_(0, ctx_slots, g * v)
     return deltas
+
+
+# ---------------------------------------------------------------------------
+# 8-bit row records: [code: 1 byte x dim][zeros to a multiple of 4][scale].
+#   int8: scale = RN(amax / 127) between 2^-126 and _INT8_TOP, code =
+#         RNE(x / scale)
+#   fp8 : scale = smallest power of two >= 2^-126 with amax <= 448 * scale,
+#         code = e4m3(x / scale), |x| at most _FP8_TOP
+# The codes are those of the exact quotients, so the records of the HIP path
+# match byte for byte.  A row with inf or NaN: NaN scale, zero codes.
+# ---------------------------------------------------------------------------
+
+_TINY = 2.0 ** -126
+_FP8_TOP = 240 * 2.0 ** 120  # the next code up stands for 2^128
+# the largest scale whose code 127 is finite (RN(FLT_MAX / 127) is one ulp up)
+_INT8_TOP = 2.6793883890187504e+36
+
+
+def cache_write(cache: torch.Tensor, values: torch.Tensor,
+                slots: Optional[torch.Tensor] = None, fmt: str = "int8",
+                unique: bool = False) -> None:
+    dim = values.shape[1]
+    if not values.shape[0]:
+        return
+    x = values.detach().float()
+    finite = torch.isfinite(x).all(1, keepdim=True)
+    x = torch.where(finite, x, 0.0)
+    amax = x.abs().amax(1, keepdim=True)
+    if fmt == "int8":
+        scale = (amax / torch.full_like(amax, 127)).clamp(_TINY, _INT8_TOP)
+        # f64 quotients: f32 ones round values next to a half onto it
+        codes = torch.round(x.double() / scale.double()).to(torch.int8)
+    else:
+        m, e = torch.frexp(amax)
+        k = torch.where(m <= 0.875, e - 9, e - 8).clamp(min=-126)
+        k = torch.where(amax > 0, k, -126)  # frexp(0) is (0, 0)
+        scale = torch.ldexp(torch.ones_like(amax), k)
+        codes = (x.clamp(-_FP8_TOP, _FP8_TOP) / scale).to(
+            torch.float8_e4m3fn)
+    scale = torch.where(finite, scale, float("nan"))
+    record = torch.zeros(x.shape[0], cache.shape[1], dtype=torch.uint8,
+                         device=x.device)
+    record[:, :dim] = codes.view(torch.uint8)
+    record[:, -4:] = scale.view(torch.uint8)
+    if slots is None:
+        cache.copy_(record)
+        return
+    slots = slots.long()
+    rows = cache.shape[0]
+    kept = (slots >= 0) & (slots < rows)
+    slots, record = slots[kept], record[kept]
+    if not unique:
+        order = torch.arange(slots.numel(), device=slots.device)
+        owner = torch.full((rows,), -1, dtype=torch.int64,
+                           device=slots.device)
+        owner.scatter_reduce_(0, slots, order, "amax")
+        last = owner[slots] == order
+        slots, record = slots[last], record[last]
+    cache[slots] = record
+
+
+def cache_read(cache: torch.Tensor, dim: int,
+               slots: Optional[torch.Tensor] = None, fmt: str = "int8",
+               dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    rows = cache.shape[0]
+    held = None
+    if slots is not None:
+        slots = slots.long()
+        if not rows:
+            return torch.zeros(slots.numel(), dim, dtype=dtype,
+                               device=cache.device)
+        held = (slots >= 0) & (slots < rows)
+        cache = cache[slots.clamp(0, rows - 1)]
+    code = torch.int8 if fmt == "int8" else torch.float8_e4m3fn
+    out = cache[:, :dim].contiguous().view(code).float() \
+        * cache[:, -4:].contiguous().view(torch.float32)
+    if held is not None:
+        out = torch.where(held[:, None], out, 0.0)
+    return out.to(dtype)

@@ -49,6 +49,7 @@ from typing import Any, Dict, Iterable, Iterator, List, Optional, Tuple
 import torch
 
 from ..api import ParameterServer, ParameterServerClient, ServerLogic, WorkerLogic
+from .. import ops
 from ..config import PSConfig
 from .partitioner import Partitioner, bucket_by_shard, make_partitioner
 from .transport import Transport, LocalTransport
@@ -321,13 +322,11 @@ class PSEngine:
                           self._queued_pulls() == 0 and
                           not self._pull_buf and not self._push_buf and
                           push_ids is None)
-        dim = self.cfg.dim
-        wire = torch.bfloat16 if self.cfg.wire_dtype == "bf16" \
-            else torch.float32
-        self._wire_out(send[2], wire)
+        wire = self._wire_spec()
+        self._wire_out(send[2])
         m.bytes_sent += self._xgmi_bytes(send)
         recv, ctrl = self.transport.alltoallv(
-            send, [(torch.int64, ()), (torch.int64, ()), (wire, (dim,))],
+            send, [(torch.int64, ()), (torch.int64, ()), wire],
             extra=[self._clock, worker_done, int(exhausted)])
         recv = self._to_device(recv)
         self._unwire(recv[2])
@@ -352,12 +351,12 @@ class PSEngine:
                     for w in range(self.world)]
         if self._answers_in_order:
             self._answer_buf = [[] for _ in range(self.world)]
-            self._wire_out(ans_vals, wire)
+            self._wire_out(ans_vals)
             m.bytes_sent += self._xgmi_bytes([ans_vals])
             counts = [0 if t is None else int(t.numel())
                       for t in sent_pulls]
             back_vals = self._to_device(self.transport.alltoallv(
-                [ans_vals], [(wire, (dim,))], recv_counts=[counts]))[0]
+                [ans_vals], [wire], recv_counts=[counts]))[0]
             self._unwire(back_vals)
             for s in range(self.world):
                 if back_vals[s] is not None and back_vals[s].numel():
@@ -368,11 +367,11 @@ class PSEngine:
             ans_ids = [_concat([a for a, _ in self._answer_buf[w]])
                        for w in range(self.world)]
             self._answer_buf = [[] for _ in range(self.world)]
-            self._wire_out(ans_vals, wire)
+            self._wire_out(ans_vals)
             m.bytes_sent += self._xgmi_bytes([ans_ids, ans_vals])
             back = self._to_device(self.transport.alltoallv(
                 [ans_ids, ans_vals],
-                [(torch.int64, ()), (wire, (dim,))]))
+                [(torch.int64, ()), wire]))
             self._unwire(back[1])
             for s in range(self.world):
                 if back[0][s] is not None and back[0][s].numel():
@@ -437,21 +436,19 @@ class PSEngine:
                           not self._pull_buf and not self._push_buf and
                           push_ids is None and
                           not any(self._answer_buf))
-        dim = self.cfg.dim
-        wire = torch.bfloat16 if self.cfg.wire_dtype == "bf16" \
-            else torch.float32
-        self._wire_out(send[2], wire)
+        wire = self._wire_spec()
+        self._wire_out(send[2])
         ans_vals = [_concat([v for _, v in self._answer_buf[w]])
                     for w in range(self.world)]
-        self._wire_out(ans_vals, wire)
+        self._wire_out(ans_vals)
         chans = [send[0], send[1], send[2]]
-        specs = [(torch.int64, ()), (torch.int64, ()), (wire, (dim,))]
+        specs = [(torch.int64, ()), (torch.int64, ()), wire]
         if not self._answers_in_order:
             chans.append([_concat([a for a, _ in self._answer_buf[w]])
                           for w in range(self.world)])
             specs.append((torch.int64, ()))
         chans.append(ans_vals)
-        specs.append((wire, (dim,)))
+        specs.append(wire)
         self._answer_buf = [[] for _ in range(self.world)]
         m.bytes_sent += self._xgmi_bytes(chans)
         recv, ctrl = self.transport.alltoallv(
@@ -570,21 +567,19 @@ class PSEngine:
                           push_ids is None and
                           not any(self._answer_buf) and
                           not self._held)
-        dim = self.cfg.dim
-        wire = torch.bfloat16 if self.cfg.wire_dtype == "bf16" \
-            else torch.float32
-        self._wire_out(send[2], wire)
+        wire = self._wire_spec()
+        self._wire_out(send[2])
         ans_vals = [_concat([v for _, v in self._answer_buf[w]])
                     for w in range(self.world)]
-        self._wire_out(ans_vals, wire)
+        self._wire_out(ans_vals)
         chans = [send[0], send[1], send[2]]
-        specs = [(torch.int64, ()), (torch.int64, ()), (wire, (dim,))]
+        specs = [(torch.int64, ()), (torch.int64, ()), wire]
         if not self._answers_in_order:
             chans.append([_concat([a for a, _ in self._answer_buf[w]])
                           for w in range(self.world)])
             specs.append((torch.int64, ()))
         chans.append(ans_vals)
-        specs.append((wire, (dim,)))
+        specs.append(wire)
         self._answer_buf = [[] for _ in range(self.world)]
         m.bytes_sent += self._xgmi_bytes(chans)
 
@@ -706,22 +701,43 @@ class PSEngine:
                     total += t.numel() * t.element_size()
         return total
 
-    def _wire_out(self, chan: List[Optional[torch.Tensor]],
-                  wire: torch.dtype) -> None:
-        """Cast a payload channel to the wire dtype in place (bf16 halves
-        xGMI bytes; tables keep f32 masters, so only the wire narrows).
+    def _wire_spec(self) -> Tuple[torch.dtype, Tuple[int, ...]]:
+        """(dtype, trailing shape) of a payload row on the wire."""
+        fmt, dim = self.cfg.wire_dtype, self.cfg.dim
+        if fmt in ("int8", "fp8"):
+            return torch.uint8, (ops.record_bytes(dim),)
+        return (torch.bfloat16 if fmt == "bf16" else torch.float32), (dim,)
+
+    def _wire_out(self, chan: List[Optional[torch.Tensor]]) -> None:
+        """Narrow a payload channel to the wire dtype in place (bf16 halves
+        xGMI bytes, 8-bit row records nearly quarter them; tables keep f32
+        masters, so only the wire narrows).
         The self-addressed segment short-circuits in every transport and
         stays f32 — full precision for the 1/world local fraction."""
-        if wire is torch.float32:
+        fmt = self.cfg.wire_dtype
+        if fmt == "f32":
             return
         for d, t in enumerate(chan):
-            if t is not None and d != self.rank:
-                chan[d] = t.to(wire)
+            if t is None or d == self.rank:
+                continue
+            if fmt == "bf16":
+                chan[d] = t.to(torch.bfloat16)
+            else:
+                t = t.detach().reshape(-1, self.cfg.dim).float()
+                rec = torch.empty(t.shape[0], ops.record_bytes(self.cfg.dim),
+                                  dtype=torch.uint8, device=t.device)
+                ops.cache_write(rec, t, fmt=fmt)
+                chan[d] = rec
 
-    @staticmethod
-    def _unwire(chan: List[Optional[torch.Tensor]]) -> None:
+    def _unwire(self, chan: List[Optional[torch.Tensor]]) -> None:
+        records = self.cfg.wire_dtype in ("int8", "fp8")
         for s, t in enumerate(chan):
-            if t is not None and t.dtype is not torch.float32:
+            if t is None or t.dtype is torch.float32:
+                continue
+            if records and s != self.rank:
+                chan[s] = ops.cache_read(t, self.cfg.dim,
+                                         fmt=self.cfg.wire_dtype)
+            else:
                 chan[s] = t.float()
 
     # ------------------------------------------------------------------
