@@ -7,7 +7,7 @@ in-tree extension; a missing extension raises (never a silent fallback).
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -18,6 +18,7 @@ __all__ = [
     "gather", "apply_add", "apply_adagrad", "hash_init",
     "mf_sgd_step", "pa_step", "pa_multiclass_step", "lr_step", "sgns_step",
     "record_bytes", "row_cache", "cache_write", "cache_read",
+    "MUON_COEFFS", "orthogonalize", "apply_muon",
     "reference", "hip",
 ]
 
@@ -262,3 +263,116 @@ def cache_read(cache: torch.Tensor, dim: int,
     if _cuda(cache):
         return hip.ext().cache_read(cache, int(dim), slots, fmt, dtype)
     return reference.cache_read(cache, int(dim), slots, fmt, dtype)
+
+
+# ---------------------------------------------------------------------------
+# Muon
+# ---------------------------------------------------------------------------
+
+#: the quintic of the Muon optimiser: steep at zero, values near one after
+#: five steps (0.7 to 1.2)
+MUON_COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+def _check_chain(name: str, steps: int, coeffs: Sequence[float],
+                 eps: float) -> Tuple[float, float, float]:
+    if not 1 <= int(steps) <= 100:
+        raise ValueError(f"{name}: steps must be 1 to 100, got {steps}")
+    if len(coeffs) != 3:
+        raise ValueError(f"{name}: coeffs are (a, b, c), got {coeffs!r}")
+    if not 0 < eps < float("inf"):
+        raise ValueError(f"{name}: eps must be positive, got {eps}")
+    a, b, c = (float(v) for v in coeffs)
+    if abs(a) > 12 or abs(b) > 12 or abs(c) > 12:
+        raise ValueError(f"{name}: coefficients beyond 12, got {coeffs!r}")
+    return a, b, c
+
+
+def orthogonalize(x: torch.Tensor, steps: int = 5,
+                  coeffs: Sequence[float] = MUON_COEFFS,
+                  eps: float = 1e-7) -> torch.Tensor:
+    """The nearest (semi-)orthogonal matrices to those of ``x`` (..., m, n;
+    f32, bf16 or f16), approximately: X = x / (|x|_F + eps), then ``steps``
+    times X <- a X + (b G + c G^2) X with G = X X^T.  Singular values near
+    zero stay there, the others come near one.
+
+    Computed to f32 accuracy whatever the type, rounded once at the end; the
+    result is new and contiguous.  A matrix that holds an infinity or NaN
+    gives NaN throughout, a matrix of zeros gives zeros.  Has no gradient."""
+    if x.dim() < 2 or x.dtype not in _VALUE_TYPES:
+        raise ValueError("orthogonalize: x must be matrices of float32, "
+                         f"bfloat16 or float16, got {x.dtype} of "
+                         f"{tuple(x.shape)}")
+    a, b, c = _check_chain("orthogonalize", steps, coeffs, eps)
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("orthogonalize has no gradient: pass x.detach()")
+    if not x.numel():
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    batch = x.detach().reshape(-1, *x.shape[-2:]).contiguous()
+    if _cuda(x):
+        out = hip.ext().orthogonalize(batch, int(steps), a, b, c, float(eps))
+    else:
+        out = reference.orthogonalize(batch, int(steps), (a, b, c),
+                                      float(eps))
+    return out.view(x.shape)
+
+
+def apply_muon(table: torch.Tensor, momentum: torch.Tensor,
+               rows: torch.Tensor, grads: torch.Tensor, lr: float,
+               mu: float = 0.95, nesterov: bool = True,
+               weight_decay: float = 0.0, steps: int = 5,
+               matrix_rows: Optional[int] = None,
+               sorted_unique: bool = False,
+               coeffs: Sequence[float] = MUON_COEFFS,
+               eps: float = 1e-7) -> None:
+    """Muon apply: ``table`` (f32) is a stack of matrices of ``matrix_rows``
+    rows each (one matrix by default).  For every matrix W that ``rows``
+    names a row of, with g the sum of its rows of ``grads`` (zero where none
+    was given) and M its part of ``momentum``:
+
+        M <- mu M + g;  U = g + mu M (``nesterov``) or M
+        W <- (1 - lr weight_decay) W - lr sqrt(max(1, m / n)) O(U)
+
+    with O as :func:`orthogonalize`.  The other matrices keep W and M.  Rows
+    outside the table are left out.  Repeated rows are summed in the order
+    that they come in.  ``sorted_unique``: the caller guarantees ``rows``
+    ascending with no duplicates, so the pre-sort is skipped."""
+    a, b, c = _check_chain("apply_muon", steps, coeffs, eps)
+    if table.dim() != 2 or table.dtype != torch.float32 \
+            or momentum.shape != table.shape \
+            or momentum.dtype != torch.float32:
+        raise ValueError("apply_muon: table and momentum must be float32 of "
+                         f"one 2-D shape, got {table.dtype} of "
+                         f"{tuple(table.shape)} and {momentum.dtype} of "
+                         f"{tuple(momentum.shape)}")
+    if not table.is_contiguous() or not momentum.is_contiguous():
+        raise ValueError("apply_muon: table and momentum must be contiguous")
+    if table.numel() and table.data_ptr() == momentum.data_ptr():
+        raise ValueError("apply_muon: table and momentum are the same memory")
+    if rows.dim() != 1 or rows.dtype not in (torch.int64, torch.int32) \
+            or grads.dtype != torch.float32 \
+            or grads.shape != (rows.numel(), table.shape[1]):
+        raise ValueError("apply_muon: rows must be 1-D int64 or int32 and "
+                         "grads float32 with one row for each, got "
+                         f"{rows.dtype} of {tuple(rows.shape)} and "
+                         f"{grads.dtype} of {tuple(grads.shape)}")
+    if not table.device == momentum.device == rows.device == grads.device:
+        raise ValueError("apply_muon: operands on several devices")
+    m = table.shape[0] if matrix_rows is None else int(matrix_rows)
+    if table.shape[0] and (m < 1 or table.shape[0] % m):
+        raise ValueError(f"apply_muon: a table of {table.shape[0]} rows is "
+                         f"not a whole number of matrices of {m}")
+    if not rows.numel() or not table.numel():
+        return
+    rows, grads = rows.long().contiguous(), grads.detach().contiguous()
+    order = None
+    if not sorted_unique:
+        rows, order = torch.sort(rows, stable=True)
+    args = (lr, mu, nesterov, weight_decay, int(steps), m)
+    if _cuda(table):
+        hip.ext().apply_muon(table, momentum, rows, order, grads,
+                             *args, a, b, c, float(eps))
+        return
+    reference.apply_muon(table, momentum, rows,
+                         grads if order is None else grads[order],
+                         *args, (a, b, c), float(eps))

@@ -393,3 +393,46 @@ def cache_read(cache: torch.Tensor, dim: int,
     if held is not None:
         out = torch.where(held[:, None], out, 0.0)
     return out.to(dtype)
+
+
+# ---------------------------------------------------------------------------
+# Muon: momentum, then the update's nearest orthogonal matrix by Newton-
+# Schulz steps (X <- aX + (bG + cG^2) X, G = X X^T on the shorter side).
+# ---------------------------------------------------------------------------
+
+def orthogonalize(x: torch.Tensor, steps: int,
+                  coeffs: Tuple[float, float, float],
+                  eps: float) -> torch.Tensor:
+    """(batch, m, n) matrices; f32 whatever the type, the norm in f64."""
+    a, b, c = coeffs
+    norm = x.double().square().sum((1, 2), keepdim=True).sqrt()
+    y = (x.double() / (norm + eps)).float()
+    y = torch.where(torch.isfinite(norm), y, float("nan"))
+    tall = x.shape[1] > x.shape[2]
+    if tall:
+        y = y.mT
+    for _ in range(steps):
+        g = torch.bmm(y, y.mT)
+        y = a * y + torch.bmm(b * g + c * torch.bmm(g, g), y)
+    return (y.mT if tall else y).to(x.dtype).contiguous()
+
+
+def apply_muon(table: torch.Tensor, momentum: torch.Tensor,
+               rows: torch.Tensor, grads: torch.Tensor, lr: float,
+               mu: float, nesterov: bool, weight_decay: float, steps: int,
+               matrix_rows: int, coeffs: Tuple[float, float, float],
+               eps: float) -> None:
+    """``rows`` sorted; only the matrices that hold one of them change."""
+    m, n = matrix_rows, table.shape[1]
+    held = (rows >= 0) & (rows < table.shape[0])
+    rows, grads = rows[held], grads[held]
+    for k in torch.unique(rows // m).tolist():
+        mine = rows // m == k
+        g = torch.zeros(m, n)
+        g.index_add_(0, rows[mine] - k * m, grads[mine])
+        M = momentum[k * m:(k + 1) * m]
+        M.mul_(mu).add_(g)
+        u = g + mu * M if nesterov else M
+        step = orthogonalize(u[None], steps, coeffs, eps)[0]
+        table[k * m:(k + 1) * m].mul_(1 - lr * weight_decay).sub_(
+            lr * max(1.0, m / n) ** 0.5 * step)

@@ -11,7 +11,7 @@ of the id), updated by HIP scatter-apply kernels.
 """
 from __future__ import annotations
 
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 
@@ -26,13 +26,33 @@ class ShardedTable:
       "add"     — W[id] += delta           (reference paramUpdate = vectorSum /
                                             '+'; the worker scales by lr)
       "adagrad" — G += g^2; W -= lr*g/sqrt(G+eps)   (new capability)
+      "muon"    — for tables of weight matrices, ``matrix_rows``
+                  consecutive ids each (default: the whole table is one):
+                  M = momentum*M + g; W = (1-lr*weight_decay)*W -
+                  lr*sqrt(max(1, m/n))*O, O the orthogonalised g +
+                  momentum*M (``nesterov``) or M (ops.apply_muon).  Every
+                  push batch is one step of the matrices that it names a
+                  row of.  A matrix has to lie on one shard: with several
+                  shards use a RangePartitioner whose blocks hold whole
+                  matrices.  M is checkpointed as the accumulator.
     """
 
     def __init__(self, part: Partitioner, shard: int, dim: int,
                  device: torch.device,
                  init: Tuple[float, float] = (0.0, 0.0),
                  optimizer: str = "add", lr: float = 0.0,
-                 eps: float = 1e-8, seed: int = 0):
+                 eps: float = 1e-8, seed: int = 0,
+                 momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0,
+                 matrix_rows: Optional[int] = None):
+        if optimizer not in ("add", "adagrad", "muon"):
+            raise ValueError(f"unknown optimizer {optimizer!r}")
+        if optimizer == "muon":
+            matrix_rows = self._whole_matrices(part, shard, matrix_rows)
+        self.momentum = float(momentum)
+        self.nesterov = bool(nesterov)
+        self.weight_decay = float(weight_decay)
+        self.matrix_rows = matrix_rows
         self.part = part
         self.shard = shard
         self._full_ids: "torch.Tensor | None" = None
@@ -63,13 +83,35 @@ class ShardedTable:
                 stride = 1
             if rows:
                 ops.hash_init_rows(self.data, first, stride, lo, hi, seed)
-        if optimizer == "adagrad":
+        if optimizer in ("adagrad", "muon"):
             self.accum = torch.zeros(rows, dim, dtype=torch.float32,
                                      device=self.device)
-        elif optimizer == "add":
-            self.accum = None
         else:
-            raise ValueError(f"unknown optimizer {optimizer!r}")
+            self.accum = None
+
+    @staticmethod
+    def _whole_matrices(part: Partitioner, shard: int,
+                        matrix_rows: Optional[int]) -> int:
+        """``matrix_rows``, checked: the shard's rows are whole matrices of
+        consecutive ids."""
+        rows = part.shard_rows(shard)
+        if matrix_rows is None:
+            if part.n_shards > 1:
+                raise ValueError(
+                    "optimizer 'muon' over several shards needs matrix_rows "
+                    "(consecutive ids of one matrix)")
+            return max(1, rows)
+        m = int(matrix_rows)
+        if m < 1:
+            raise ValueError(f"matrix_rows must be at least 1, got {m}")
+        if rows:
+            ends = part.global_id(shard, torch.tensor([0, rows - 1])).tolist()
+            if ends[1] - ends[0] != rows - 1 or ends[0] % m or rows % m:
+                raise ValueError(
+                    f"shard {shard} does not hold whole matrices of {m} "
+                    "consecutive ids: use a RangePartitioner whose blocks "
+                    "are multiples of matrix_rows")
+        return m
 
     # -- server-side ops (K3 gather / K1 sgd apply / K2 adagrad apply) ----
 
@@ -116,6 +158,13 @@ class ShardedTable:
         rows = self.part.local_row(ids)
         if self.optimizer == "add":
             ops.apply_add(self.data, rows, deltas, unique)
+        elif self.optimizer == "muon":
+            ops.apply_muon(self.data, self.accum, rows.to(self.device),
+                           deltas, self.lr, mu=self.momentum,
+                           nesterov=self.nesterov,
+                           weight_decay=self.weight_decay,
+                           matrix_rows=self.matrix_rows,
+                           sorted_unique=unique)
         else:
             # `unique` batches arrive as sorted unique pulled ids, and
             # both partitioners are monotone per shard, so the local

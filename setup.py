@@ -20,7 +20,8 @@ setup(
     ext_modules=[
         CUDAExtension(
             name="flink_parameter_server_amd._C",
-            sources=["csrc/ps_kernels.hip", "csrc/row_cache.hip"],
+            sources=["csrc/ps_kernels.hip", "csrc/row_cache.hip",
+                     "csrc/muon.hip"],
             depends=["csrc/ops.h"],
             extra_compile_args={
                 "cxx": ["-O3"],
