@@ -22,6 +22,9 @@
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "ops.h"
 
 namespace {
@@ -57,10 +60,73 @@ __device__ inline __hip_bfloat16 from_f32(float v) {
   return __float2bfloat16(v);
 }
 
-template <typename S>
-__device__ inline int64_t slot_of(const S* slots, int64_t j) {
-  return slots ? (int64_t)slots[j] : j;
+// Four neighbouring values at any address that a T may have: the memory
+// path takes vectors that are aligned to their elements.
+template <typename T>
+struct Bits;
+template <>
+struct Bits<float> { using Raw = float; };
+template <>
+struct Bits<__half> { using Raw = uint16_t; };
+template <>
+struct Bits<__hip_bfloat16> { using Raw = uint16_t; };
+
+template <typename T>
+struct Quad {
+  using Raw = typename Bits<T>::Raw;
+  typedef Raw Vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  Vec v;
+  __device__ inline void load(const T* at) { v = *(const Vec*)at; }
+  __device__ inline void store(T* at) const { *(Vec*)at = v; }
+  __device__ inline T get(int i) const {
+    Raw r = v[i];
+    return *(T*)&r;
+  }
+  __device__ inline void set(int i, T t) { v[i] = *(Raw*)&t; }
+};
+
+// The first `held` (1 to 4) of four values, zeros after them.
+template <typename T>
+__device__ inline float4 load_quad(const T* at, int held) {
+  float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (held >= 4) {
+    Quad<T> q;
+    q.load(at);
+    f = make_float4(to_f32(q.get(0)), to_f32(q.get(1)), to_f32(q.get(2)),
+                    to_f32(q.get(3)));
+  } else {
+    if (held > 0) f.x = to_f32(at[0]);
+    if (held > 1) f.y = to_f32(at[1]);
+    if (held > 2) f.z = to_f32(at[2]);
+  }
+  return f;
 }
+
+template <typename T>
+__device__ inline void store_quad(T* at, float4 f, int held) {
+  Quad<T> q;
+  q.set(0, from_f32<T>(f.x));
+  q.set(1, from_f32<T>(f.y));
+  q.set(2, from_f32<T>(f.z));
+  q.set(3, from_f32<T>(f.w));
+  if (held >= 4) {
+    q.store(at);
+  } else {
+    if (held > 0) at[0] = q.get(0);
+    if (held > 1) at[1] = q.get(1);
+    if (held > 2) at[2] = q.get(2);
+  }
+}
+
+// int64, int32 or no slots (row j's is j)
+struct Slots {
+  const void* at;
+  bool wide;
+  __device__ inline int64_t operator[](int64_t j) const {
+    if (!at) return j;
+    return wide ? ((const int64_t*)at)[j] : ((const int32_t*)at)[j];
+  }
+};
 
 // |x| as an ordered integer: finite < inf < NaN, so the largest one of a
 // row also says whether the row is finite.
@@ -93,126 +159,279 @@ __device__ inline int code_int8(float x, float s, float inv) {
   return (int)q;
 }
 
-__device__ inline uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int o = WAVE / 2; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+__device__ inline uint32_t quad_magnitude(float4 f) {
+  return max(max(magnitude(f.x), magnitude(f.y)),
+             max(magnitude(f.z), magnitude(f.w)));
+}
+
+__device__ inline uint32_t group_max(uint32_t v, int group) {
+  for (int o = group / 2; o; o >>= 1)
+    v = max(v, (uint32_t)__shfl_xor((int)v, o));
   return v;
 }
 
+template <bool FP8>
+__device__ inline uint32_t encode(float4 f, float s, float inv) {
+  if (s != s) return 0;  // the row is not finite
+  if (FP8) {
+    auto part = [&](float x) {
+      return __builtin_amdgcn_fmed3f(x, -FP8_TOP, FP8_TOP) * inv;
+    };
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(part(f.x), part(f.y), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(part(f.z), part(f.w), w,
+                                                     true);
+  }
+  return (uint32_t)(code_int8(f.x, s, inv) & 255) |
+         (uint32_t)(code_int8(f.y, s, inv) & 255) << 8 |
+         (uint32_t)(code_int8(f.z, s, inv) & 255) << 16 |
+         (uint32_t)code_int8(f.w, s, inv) << 24;
+}
+
+template <bool FP8>
+__device__ inline float4 decode(uint32_t w, float s) {
+  if (FP8)
+    return make_float4(__builtin_amdgcn_cvt_f32_fp8((int)w, 0) * s,
+                       __builtin_amdgcn_cvt_f32_fp8((int)w, 1) * s,
+                       __builtin_amdgcn_cvt_f32_fp8((int)w, 2) * s,
+                       __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * s);
+  return make_float4((float)(int8_t)w * s, (float)(int8_t)(w >> 8) * s,
+                     (float)(int8_t)(w >> 16) * s,
+                     (float)(int8_t)(w >> 24) * s);
+}
+
 // The last of the writes to a slot wins, whatever the order that they run in.
-template <typename S>
-__global__ __launch_bounds__(256) void k_cache_owner(
-    int* __restrict__ owner, const S* __restrict__ slots, int64_t n,
-    int64_t rows) {
+__global__ __launch_bounds__(256) void k_cache_owner(int* __restrict__ owner,
+                                                     Slots slots, int64_t n,
+                                                     int64_t rows) {
   for (int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x; j < n;
        j += (int64_t)gridDim.x * 256) {
-    int64_t s = (int64_t)slots[j];
+    int64_t s = slots[j];
     if (s >= 0 && s < rows) atomicMax(owner + s, (int)j);
   }
 }
 
-// One wave a row: the row's largest magnitude, then its codes.
-template <typename T, typename S, bool FP8>
+// `group` lanes (a power of two) take ROWS rows at a time; a lane holds QUADS
+// quads of each in registers, so that the values are read once, and all the
+// loads of a turn are under way before the first is used.
+template <typename T, bool FP8, int QUADS, int ROWS>
 __global__ __launch_bounds__(256) void k_cache_write(
     uint8_t* __restrict__ cache, int64_t cache_stride,
-    const T* __restrict__ values, int64_t value_stride,
-    const S* __restrict__ slots, const int* __restrict__ owner, int64_t n,
-    int64_t dim, int64_t rows) {
+    const T* __restrict__ values, int64_t value_stride, Slots slots,
+    const int* __restrict__ owner, int64_t n, int dim, int64_t rows,
+    int group) {
+  const int lane = threadIdx.x & (group - 1);
+  const int per_block = 256 / group;
+  const int quads = (dim + 3) / 4;
+  for (int64_t j0 = ((int64_t)blockIdx.x * per_block + threadIdx.x / group) *
+                    ROWS;
+       j0 < n; j0 += (int64_t)gridDim.x * per_block * ROWS) {
+    int64_t slot[ROWS];
+    float4 x[ROWS][QUADS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      slot[r] = j0 + r < n ? slots[j0 + r] : -1;
+      if (slot[r] >= rows) slot[r] = -1;
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (owner && slot[r] >= 0 && owner[slot[r]] != (int)(j0 + r))
+        slot[r] = -1;
+#pragma unroll
+      for (int i = 0; i < QUADS; ++i) {
+        const int q = lane + i * group;
+        x[r][i] = load_quad(values + (j0 + r) * value_stride + q * 4,
+                            slot[r] < 0 ? 0 : dim - q * 4);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < QUADS; ++i) top = max(top, quad_magnitude(x[r][i]));
+      const float s = scale_of<FP8>(group_max(top, group));
+      const float inv = 1.0f / s;
+      if (slot[r] < 0) continue;
+      uint32_t* out = (uint32_t*)(cache + slot[r] * cache_stride);
+#pragma unroll
+      for (int i = 0; i < QUADS; ++i) {
+        const int q = lane + i * group;
+        if (q < quads) out[q] = encode<FP8>(x[r][i], s, inv);
+      }
+      if (lane == 0) out[quads] = __float_as_uint(s);
+    }
+  }
+}
+
+// Rows too long for registers: a wave a row, which it reads twice.
+template <typename T, bool FP8>
+__global__ __launch_bounds__(256) void k_cache_write_long(
+    uint8_t* __restrict__ cache, int64_t cache_stride,
+    const T* __restrict__ values, int64_t value_stride, Slots slots,
+    const int* __restrict__ owner, int64_t n, int64_t dim, int64_t rows) {
   const int lane = threadIdx.x % WAVE;
-  const int64_t waves = (int64_t)gridDim.x * (256 / WAVE);
-  const int64_t padded = (dim + 3) / 4 * 4;
-  for (int64_t j = (int64_t)blockIdx.x * (256 / WAVE) + threadIdx.x / WAVE;
-       j < n; j += waves) {
-    int64_t slot = slot_of(slots, j);
+  const int64_t quads = (dim + 3) / 4;
+  for (int64_t j = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE; j < n;
+       j += (int64_t)gridDim.x * 4) {
+    const int64_t slot = slots[j];
     if (slot < 0 || slot >= rows) continue;
     if (owner && owner[slot] != (int)j) continue;
     const T* x = values + j * value_stride;
-    uint8_t* out = cache + slot * cache_stride;
+    uint32_t* out = (uint32_t*)(cache + slot * cache_stride);
     uint32_t top = 0;
-    for (int64_t c = lane; c < dim; c += WAVE)
-      top = max(top, magnitude(to_f32(x[c])));
-    const float s = scale_of<FP8>(wave_max(top));
-    const bool finite = s == s;
+    for (int64_t q = lane; q < quads; q += WAVE)
+      top = max(top, quad_magnitude(load_quad(
+                         x + q * 4, (int)min(dim - q * 4, (int64_t)4))));
+    const float s = scale_of<FP8>(group_max(top, WAVE));
     const float inv = 1.0f / s;
-    for (int64_t c = lane; c < padded; c += WAVE) {
-      uint8_t code = 0;
-      if (c < dim && finite) {
-        float v = to_f32(x[c]);
-        if (FP8)
-          code = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(
-              __builtin_amdgcn_fmed3f(v, -FP8_TOP, FP8_TOP) * inv, 0.0f, 0,
-              false);
-        else
-          code = (uint8_t)code_int8(v, s, inv);
-      }
-      out[c] = code;
-    }
-    if (lane == 0) *(float*)(out + padded) = s;
+    for (int64_t q = lane; q < quads; q += WAVE)
+      out[q] = encode<FP8>(
+          load_quad(x + q * 4, (int)min(dim - q * 4, (int64_t)4)), s, inv);
+    if (lane == 0) out[quads] = __float_as_uint(s);
   }
 }
 
-template <typename T, typename S, bool FP8>
+template <typename T, bool FP8, int QUADS, int ROWS>
 __global__ __launch_bounds__(256) void k_cache_read(
     T* __restrict__ out, const uint8_t* __restrict__ cache,
-    int64_t cache_stride, const S* __restrict__ slots, int64_t n, int64_t dim,
-    int64_t rows) {
-  const int lane = threadIdx.x % WAVE;
-  const int64_t waves = (int64_t)gridDim.x * (256 / WAVE);
-  const int64_t padded = (dim + 3) / 4 * 4;
-  for (int64_t j = (int64_t)blockIdx.x * (256 / WAVE) + threadIdx.x / WAVE;
-       j < n; j += waves) {
-    int64_t slot = slot_of(slots, j);
-    const bool held = slot >= 0 && slot < rows;
-    const uint8_t* rec = cache + (held ? slot : 0) * cache_stride;
-    const float s = held ? *(const float*)(rec + padded) : 0.0f;
-    for (int64_t c = lane; c < dim; c += WAVE) {
-      float v = 0.0f;
-      if (held) {
-        uint8_t code = rec[c];
-        v = (FP8 ? __builtin_amdgcn_cvt_f32_fp8((int)code, 0)
-                 : (float)(int8_t)code) * s;
+    int64_t cache_stride, Slots slots, int64_t n, int dim, int64_t rows,
+    int group) {
+  const int lane = threadIdx.x & (group - 1);
+  const int per_block = 256 / group;
+  const int quads = (dim + 3) / 4;
+  for (int64_t j0 = ((int64_t)blockIdx.x * per_block + threadIdx.x / group) *
+                    ROWS;
+       j0 < n; j0 += (int64_t)gridDim.x * per_block * ROWS) {
+    int64_t slot[ROWS];
+    uint32_t w[ROWS][QUADS];
+    float s[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      slot[r] = j0 + r < n ? slots[j0 + r] : -1;
+      if (slot[r] >= rows) slot[r] = -1;
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      // zeros for padding
+      const uint32_t* rec = (const uint32_t*)(cache + slot[r] * cache_stride);
+#pragma unroll
+      for (int i = 0; i < QUADS; ++i) {
+        const int q = lane + i * group;
+        w[r][i] = slot[r] >= 0 && q < quads ? rec[q] : 0;
       }
-      out[j * dim + c] = from_f32<T>(v);
+      s[r] = slot[r] >= 0 ? __uint_as_float(rec[quads]) : 0.0f;
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (j0 + r >= n) continue;
+#pragma unroll
+      for (int i = 0; i < QUADS; ++i) {
+        const int q = lane + i * group;
+        store_quad(out + (j0 + r) * dim + q * 4, decode<FP8>(w[r][i], s[r]),
+                   dim - q * 4);
+      }
     }
   }
 }
 
-int grid_of(int64_t waves) {
-  int64_t g = (waves + 3) / 4;
-  return (int)(g < 1 ? 1 : (g > 4096 ? 4096 : g));
+template <typename T, bool FP8>
+__global__ __launch_bounds__(256) void k_cache_read_long(
+    T* __restrict__ out, const uint8_t* __restrict__ cache,
+    int64_t cache_stride, Slots slots, int64_t n, int64_t dim, int64_t rows) {
+  const int lane = threadIdx.x % WAVE;
+  const int64_t quads = (dim + 3) / 4;
+  for (int64_t j = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE; j < n;
+       j += (int64_t)gridDim.x * 4) {
+    const int64_t slot = slots[j];
+    const bool held = slot >= 0 && slot < rows;
+    const uint32_t* rec = (const uint32_t*)(cache + (held ? slot : 0) *
+                                                        cache_stride);
+    const float s = held ? __uint_as_float(rec[quads]) : 0.0f;
+    for (int64_t q = lane; q < quads; q += WAVE)
+      store_quad(out + j * dim + q * 4, decode<FP8>(held ? rec[q] : 0, s),
+                 (int)min(dim - q * 4, (int64_t)4));
+  }
 }
 
-template <typename T, typename S>
-void launch_write(at::Tensor& cache, const at::Tensor& values, const S* slots,
-                  const int* owner, bool fp8, hipStream_t stream) {
-  int64_t n = values.size(0), dim = values.size(1);
-  auto* kfn = fp8 ? k_cache_write<T, S, true> : k_cache_write<T, S, false>;
-  hipLaunchKernelGGL(kfn, dim3(grid_of(n)), dim3(256), 0, stream,
-                     cache.data_ptr<uint8_t>(), cache.stride(0),
-                     (const T*)values.data_ptr(), values.stride(0), slots,
-                     owner, n, dim, cache.size(0));
+int grid_of(int64_t blocks) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(blocks, 4096));
 }
 
-template <typename T, typename S>
-void launch_read(at::Tensor& out, const at::Tensor& cache, const S* slots,
-                 bool fp8, hipStream_t stream) {
-  int64_t n = out.size(0), dim = out.size(1);
-  auto* kfn = fp8 ? k_cache_read<T, S, true> : k_cache_read<T, S, false>;
-  hipLaunchKernelGGL(kfn, dim3(grid_of(n)), dim3(256), 0, stream,
-                     (T*)out.data_ptr(), cache.data_ptr<uint8_t>(),
-                     cache.stride(0), slots, n, dim, cache.size(0));
+// How lanes share a row: `group` lanes of `quads` quads each, 0 quads for a
+// row too long for registers.
+struct Share { int group, quads; };
+
+Share share_of(int64_t dim) {
+  const int64_t need = (dim + 3) / 4;
+  if (need > WAVE * 8) return {WAVE, 0};
+  int group = 1, quads = 1;
+  while (group < 32 && group < need) group *= 2;
+  while (group * quads < need && quads < 4) quads *= 2;
+  while (group * quads < need && group < WAVE) group *= 2;
+  while (group * quads < need) quads *= 2;
+  return {group, quads};
 }
 
-// f(T{}, S{}) for the value type and the slot type
-template <typename F>
-void by_types(at::ScalarType t, bool wide, F f) {
-  auto slots = [&](auto v) {
-    if (wide) f(v, int64_t{}); else f(v, int32_t{});
+template <typename T, bool FP8>
+void launch_write(at::Tensor& cache, const at::Tensor& values, Slots slots,
+                  const int* owner, hipStream_t stream) {
+  const int64_t n = values.size(0), dim = values.size(1);
+  const Share sh = share_of(dim);
+  const T* x = (const T*)values.data_ptr();
+  uint8_t* out = cache.data_ptr<uint8_t>();
+  auto go = [&](auto* kfn, int rows) {
+    const int64_t per = (int64_t)(256 / sh.group) * rows;
+    hipLaunchKernelGGL(kfn, dim3(grid_of((n + per - 1) / per)), dim3(256), 0,
+                       stream, out, cache.stride(0), x, values.stride(0),
+                       slots, owner, n, (int)dim, cache.size(0), sh.group);
   };
-  if (t == at::kFloat) slots(float{});
-  else if (t == at::kHalf) slots(__half{});
-  else if (t == at::kBFloat16) slots(__hip_bfloat16{});
+  if (sh.quads == 1) go(k_cache_write<T, FP8, 1, 4>, 4);
+  else if (sh.quads == 2) go(k_cache_write<T, FP8, 2, 2>, 2);
+  else if (sh.quads == 4) go(k_cache_write<T, FP8, 4, 1>, 1);
+  else if (sh.quads == 8) go(k_cache_write<T, FP8, 8, 1>, 1);
+  else
+    hipLaunchKernelGGL((k_cache_write_long<T, FP8>), dim3(grid_of((n + 3) / 4)),
+                       dim3(256), 0, stream, out, cache.stride(0), x,
+                       values.stride(0), slots, owner, n, dim, cache.size(0));
+}
+
+template <typename T, bool FP8>
+void launch_read(at::Tensor& out, const at::Tensor& cache, Slots slots,
+                 hipStream_t stream) {
+  const int64_t n = out.size(0), dim = out.size(1);
+  const Share sh = share_of(dim);
+  T* to = (T*)out.data_ptr();
+  const uint8_t* from = cache.data_ptr<uint8_t>();
+  auto go = [&](auto* kfn, int rows) {
+    const int64_t per = (int64_t)(256 / sh.group) * rows;
+    hipLaunchKernelGGL(kfn, dim3(grid_of((n + per - 1) / per)), dim3(256), 0,
+                       stream, to, from, cache.stride(0), slots, n, (int)dim,
+                       cache.size(0), sh.group);
+  };
+  if (sh.quads == 1) go(k_cache_read<T, FP8, 1, 4>, 4);
+  else if (sh.quads == 2) go(k_cache_read<T, FP8, 2, 2>, 2);
+  else if (sh.quads == 4) go(k_cache_read<T, FP8, 4, 1>, 1);
+  else if (sh.quads == 8) go(k_cache_read<T, FP8, 8, 1>, 1);
+  else
+    hipLaunchKernelGGL((k_cache_read_long<T, FP8>), dim3(grid_of((n + 3) / 4)),
+                       dim3(256), 0, stream, to, from, cache.stride(0), slots,
+                       n, dim, cache.size(0));
+}
+
+// f(T{}, std::bool_constant<FP8>{}) for the value type and the format
+template <typename F>
+void by_types(at::ScalarType t, bool fp8, F f) {
+  auto formats = [&](auto v) {
+    if (fp8) f(v, std::true_type{}); else f(v, std::false_type{});
+  };
+  if (t == at::kFloat) formats(float{});
+  else if (t == at::kHalf) formats(__half{});
+  else if (t == at::kBFloat16) formats(__hip_bfloat16{});
   else TORCH_CHECK(false, "values must be float32, bfloat16 or float16");
+}
+
+Slots slots_of(const c10::optional<at::Tensor>& slots) {
+  if (!slots) return {nullptr, false};
+  return {slots->data_ptr(), slots->scalar_type() == at::kLong};
 }
 
 bool is_fp8(const std::string& fmt) {
@@ -266,18 +485,14 @@ void cache_write(at::Tensor cache, at::Tensor values,
   at::Tensor owner;
   if (slots && !unique)
     owner = at::full({cache.size(0)}, -1, cache.options().dtype(at::kInt));
-  by_types(values.scalar_type(),
-           slots && slots->scalar_type() == at::kLong, [&](auto t, auto s) {
-    using T = decltype(t);
-    using S = decltype(s);
-    const S* at_ = slots ? (const S*)slots->data_ptr() : nullptr;
-    if (owner.defined())
-      hipLaunchKernelGGL(k_cache_owner<S>, dim3(grid_of(n / WAVE + 1)),
-                         dim3(256), 0, stream, owner.data_ptr<int>(), at_, n,
-                         cache.size(0));
-    launch_write<T, S>(cache, values, at_,
-                       owner.defined() ? owner.data_ptr<int>() : nullptr, fp8,
-                       stream);
+  const Slots at_ = slots_of(slots);
+  int* own = owner.defined() ? owner.data_ptr<int>() : nullptr;
+  if (own)
+    hipLaunchKernelGGL(k_cache_owner, dim3(grid_of((n + 255) / 256)),
+                       dim3(256), 0, stream, own, at_, n, cache.size(0));
+  by_types(values.scalar_type(), fp8, [&](auto t, auto f) {
+    launch_write<decltype(t), decltype(f)::value>(cache, values, at_, own,
+                                                  stream);
   });
 }
 
@@ -293,13 +508,9 @@ at::Tensor cache_read(at::Tensor cache, int64_t dim,
   if (!n) return out;
   if (!cache.size(0)) return out.zero_();
   hipStream_t stream = at::hip::getCurrentHIPStream().stream();
-  by_types(dtype, slots && slots->scalar_type() == at::kLong,
-           [&](auto t, auto s) {
-    using T = decltype(t);
-    using S = decltype(s);
-    launch_read<T, S>(out, cache,
-                      slots ? (const S*)slots->data_ptr() : nullptr, fp8,
-                      stream);
+  by_types(dtype, fp8, [&](auto t, auto f) {
+    launch_read<decltype(t), decltype(f)::value>(out, cache, slots_of(slots),
+                                                 stream);
   });
   return out;
 }
