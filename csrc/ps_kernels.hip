@@ -2312,6 +2312,14 @@ std::vector<torch::Tensor> pa_multiclass_step(
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  // refused arguments: ValueError, as the CPU path raises it
+  py::register_local_exception_translator([](std::exception_ptr p) {
+    try {
+      if (p) std::rethrow_exception(p);
+    } catch (const c10::ValueError& e) {
+      PyErr_SetString(PyExc_ValueError, e.what_without_backtrace());
+    }
+  });
   m.def("gather", &gather, "K3 ps_gather");
   m.def("apply_add", &apply_add, "K1 ps_apply_sgd (delta add)",
         py::arg("table"), py::arg("rows"), py::arg("deltas"),

@@ -18,14 +18,14 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
+#include <c10/core/GradMode.h>
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <type_traits>
 
 #include "ops.h"
+#include "quads.h"
 
 namespace {
 
@@ -34,89 +34,6 @@ constexpr float TINY = 0x1p-126f;  // the smallest normal f32
 constexpr float FP8_TOP = 0x1.ep+127f;  // 240 * 2^120: the next code is 2^128
 // The largest scale whose code 127 is finite; RN(FLT_MAX / 127) is one ulp up.
 constexpr float INT8_TOP = 0x1.020406p+121f;
-
-template <typename T>
-__device__ inline float to_f32(T v);
-template <>
-__device__ inline float to_f32(float v) { return v; }
-template <>
-__device__ inline float to_f32(__half v) { return __half2float(v); }
-template <>
-__device__ inline float to_f32(__hip_bfloat16 v) { return __bfloat162float(v); }
-
-template <typename T>
-__device__ inline T from_f32(float v);
-template <>
-__device__ inline float from_f32(float v) { return v; }
-template <>
-__device__ inline __half from_f32(float v) {
-  // Keeps the product's own rounding to f32: fused with the conversion it
-  // would round once, and differ from every other path in a last place.
-  asm volatile("" : "+v"(v));
-  return __float2half_rn(v);
-}
-template <>
-__device__ inline __hip_bfloat16 from_f32(float v) {
-  return __float2bfloat16(v);
-}
-
-// Four neighbouring values at any address that a T may have: the memory
-// path takes vectors that are aligned to their elements.
-template <typename T>
-struct Bits;
-template <>
-struct Bits<float> { using Raw = float; };
-template <>
-struct Bits<__half> { using Raw = uint16_t; };
-template <>
-struct Bits<__hip_bfloat16> { using Raw = uint16_t; };
-
-template <typename T>
-struct Quad {
-  using Raw = typename Bits<T>::Raw;
-  typedef Raw Vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-  Vec v;
-  __device__ inline void load(const T* at) { v = *(const Vec*)at; }
-  __device__ inline void store(T* at) const { *(Vec*)at = v; }
-  __device__ inline T get(int i) const {
-    Raw r = v[i];
-    return *(T*)&r;
-  }
-  __device__ inline void set(int i, T t) { v[i] = *(Raw*)&t; }
-};
-
-// The first `held` (1 to 4) of four values, zeros after them.
-template <typename T>
-__device__ inline float4 load_quad(const T* at, int held) {
-  float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (held >= 4) {
-    Quad<T> q;
-    q.load(at);
-    f = make_float4(to_f32(q.get(0)), to_f32(q.get(1)), to_f32(q.get(2)),
-                    to_f32(q.get(3)));
-  } else {
-    if (held > 0) f.x = to_f32(at[0]);
-    if (held > 1) f.y = to_f32(at[1]);
-    if (held > 2) f.z = to_f32(at[2]);
-  }
-  return f;
-}
-
-template <typename T>
-__device__ inline void store_quad(T* at, float4 f, int held) {
-  Quad<T> q;
-  q.set(0, from_f32<T>(f.x));
-  q.set(1, from_f32<T>(f.y));
-  q.set(2, from_f32<T>(f.z));
-  q.set(3, from_f32<T>(f.w));
-  if (held >= 4) {
-    q.store(at);
-  } else {
-    if (held > 0) at[0] = q.get(0);
-    if (held > 1) at[1] = q.get(1);
-    if (held > 2) at[2] = q.get(2);
-  }
-}
 
 // int64, int32 or no slots (row j's is j)
 struct Slots {
@@ -279,13 +196,11 @@ __global__ __launch_bounds__(256) void k_cache_write_long(
     uint32_t* out = (uint32_t*)(cache + slot * cache_stride);
     uint32_t top = 0;
     for (int64_t q = lane; q < quads; q += WAVE)
-      top = max(top, quad_magnitude(load_quad(
-                         x + q * 4, (int)min(dim - q * 4, (int64_t)4))));
+      top = max(top, quad_magnitude(load_quad(x + q * 4, dim - q * 4)));
     const float s = scale_of<FP8>(group_max(top, WAVE));
     const float inv = 1.0f / s;
     for (int64_t q = lane; q < quads; q += WAVE)
-      out[q] = encode<FP8>(
-          load_quad(x + q * 4, (int)min(dim - q * 4, (int64_t)4)), s, inv);
+      out[q] = encode<FP8>(load_quad(x + q * 4, dim - q * 4), s, inv);
     if (lane == 0) out[quads] = __float_as_uint(s);
   }
 }
@@ -348,7 +263,7 @@ __global__ __launch_bounds__(256) void k_cache_read_long(
     const float s = held ? __uint_as_float(rec[quads]) : 0.0f;
     for (int64_t q = lane; q < quads; q += WAVE)
       store_quad(out + j * dim + q * 4, decode<FP8>(held ? rec[q] : 0, s),
-                 (int)min(dim - q * 4, (int64_t)4));
+                 dim - q * 4);
   }
 }
 
@@ -435,30 +350,37 @@ Slots slots_of(const c10::optional<at::Tensor>& slots) {
 }
 
 bool is_fp8(const std::string& fmt) {
-  TORCH_CHECK(fmt == "int8" || fmt == "fp8", "unknown row format ", fmt);
+  TORCH_CHECK_VALUE(fmt == "int8" || fmt == "fp8", "unknown row format '",
+                    fmt, "'");
   return fmt == "fp8";
 }
 
-void check_cache(const at::Tensor& cache, int64_t dim) {
-  TORCH_CHECK(cache.is_cuda(), "cache must be a device tensor");
-  TORCH_CHECK(cache.dim() == 2 && cache.scalar_type() == at::kByte,
-              "cache must be a 2-D uint8 tensor");
-  TORCH_CHECK(dim >= 1 && cache.size(1) == (dim + 3) / 4 * 4 + 4,
-              "cache records do not hold rows of ", dim, " values");
-  TORCH_CHECK(cache.stride(1) == 1 && cache.stride(0) % 4 == 0 &&
-                  (uintptr_t)cache.data_ptr() % 4 == 0,
-              "cache records must be contiguous and 4-byte aligned");
+bool is_value_type(at::ScalarType t) {
+  return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf;
 }
 
-void check_slots(const c10::optional<at::Tensor>& slots, int64_t n,
-                 const at::Tensor& cache) {
-  if (!slots) return;
-  TORCH_CHECK(slots->device() == cache.device() && slots->is_contiguous() &&
-                  slots->numel() == n &&
-                  (slots->scalar_type() == at::kLong ||
-                   slots->scalar_type() == at::kInt),
-              "slots must be n contiguous int64 or int32 on the cache's "
-              "device");
+// ops/reference.py refuses the same on the CPU.
+void check_records(const char* name, const at::Tensor& cache, int64_t dim,
+                   const c10::optional<at::Tensor>& slots) {
+  TORCH_CHECK_VALUE(
+      dim >= 1 && cache.scalar_type() == at::kByte && cache.dim() == 2 &&
+          cache.size(1) == (dim + 3) / 4 * 4 + 4,
+      name, ": the cache of rows of ", dim,
+      " values is uint8 of shape (rows, record_bytes(", dim, ")), got ",
+      cache.scalar_type(), " of ", cache.sizes());
+  TORCH_CHECK_VALUE(!cache.size(0) ||
+                        (cache.stride(1) == 1 && cache.stride(0) % 4 == 0 &&
+                         (uintptr_t)cache.data_ptr() % 4 == 0),
+                    name,
+                    ": cache records must be contiguous and 4-byte aligned");
+  if (slots)
+    TORCH_CHECK_VALUE((slots->scalar_type() == at::kLong ||
+                       slots->scalar_type() == at::kInt) &&
+                          slots->dim() == 1 &&
+                          slots->device() == cache.device(),
+                      name, ": slots must be 1-D int64 or int32 on the "
+                      "cache's device, got ", slots->scalar_type(), " of ",
+                      slots->sizes(), " on ", slots->device());
 }
 
 }  // namespace
@@ -467,21 +389,29 @@ void cache_write(at::Tensor cache, at::Tensor values,
                  c10::optional<at::Tensor> slots, const std::string& fmt,
                  bool unique) {
   const bool fp8 = is_fp8(fmt);
-  TORCH_CHECK(values.dim() == 2 && values.device() == cache.device(),
-              "values must be 2-D on the cache's device");
+  TORCH_CHECK_VALUE(values.dim() == 2 && is_value_type(values.scalar_type()) &&
+                        values.device() == cache.device(),
+                    "cache_write: values must be 2-D float32, bfloat16 or "
+                    "float16 on the cache's device, got ",
+                    values.scalar_type(), " of ", values.sizes(), " on ",
+                    values.device());
+  check_records("cache_write", cache, values.size(1), slots);
   const int64_t n = values.size(0);
-  check_cache(cache, values.size(1));
-  check_slots(slots, n, cache);
-  TORCH_CHECK(values.stride(1) == 1 || values.size(1) == 1,
-              "rows of values must be contiguous");
-  TORCH_CHECK(slots || n == cache.size(0), "without slots there is one "
-              "record for each row of values");
-  TORCH_CHECK(cache.size(0) < 2 || cache.stride(0) >= cache.size(1),
-              "cache records must not overlap");
-  TORCH_CHECK(n < (int64_t{1} << 31), "too many rows in one write");
+  TORCH_CHECK_VALUE(n == (slots ? slots->numel() : cache.size(0)),
+                    "cache_write: ", n, " rows of values for ",
+                    slots ? slots->numel() : cache.size(0),
+                    slots ? " slots" : " records");
+  TORCH_CHECK_VALUE(cache.size(0) < 2 || cache.stride(0) >= cache.size(1),
+                    "cache_write: cache records must not overlap");
+  TORCH_CHECK_VALUE(n < (int64_t{1} << 31),
+                    "cache_write: 2^31 rows or more in one write");
+  TORCH_CHECK(!(values.requires_grad() && c10::GradMode::is_enabled()),
+              "cache_write has no gradient: pass values.detach()");
   if (!n) return;
   c10::DeviceGuard guard(cache.device());
   hipStream_t stream = at::hip::getCurrentHIPStream().stream();
+  if (values.stride(1) != 1) values = values.contiguous();
+  if (slots) slots = slots->contiguous();
   at::Tensor owner;
   if (slots && !unique)
     owner = at::full({cache.size(0)}, -1, cache.options().dtype(at::kInt));
@@ -500,10 +430,12 @@ at::Tensor cache_read(at::Tensor cache, int64_t dim,
                       c10::optional<at::Tensor> slots, const std::string& fmt,
                       at::ScalarType dtype) {
   const bool fp8 = is_fp8(fmt);
-  check_cache(cache, dim);
+  check_records("cache_read", cache, dim, slots);
+  TORCH_CHECK_VALUE(is_value_type(dtype), "cache_read: dtype must be float32, "
+                    "bfloat16 or float16, got ", dtype);
   const int64_t n = slots ? slots->numel() : cache.size(0);
-  check_slots(slots, n, cache);
   c10::DeviceGuard guard(cache.device());
+  if (slots) slots = slots->contiguous();
   auto out = at::empty({n, dim}, cache.options().dtype(dtype));
   if (!n) return out;
   if (!cache.size(0)) return out.zero_();

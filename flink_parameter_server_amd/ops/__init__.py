@@ -183,31 +183,6 @@ def row_cache(rows: int, dim: int,
                        device=device)
 
 
-def _check_records(name: str, cache: torch.Tensor, dim: int,
-                   slots: Optional[torch.Tensor], fmt: str) -> None:
-    if fmt not in ("int8", "fp8"):
-        raise ValueError(f"{name}: unknown row format {fmt!r}")
-    if dim < 1:
-        raise ValueError(f"{name}: dim must be at least 1, got {dim}")
-    if cache.dtype != torch.uint8 or cache.dim() != 2 \
-            or cache.shape[1] != record_bytes(dim):
-        raise ValueError(
-            f"{name}: the cache of rows of {dim} values is uint8 of shape "
-            f"(rows, {record_bytes(dim)}), got {cache.dtype} of "
-            f"{tuple(cache.shape)}")
-    if cache.shape[0] and (cache.stride(1) != 1 or cache.stride(0) % 4
-                           or cache.data_ptr() % 4):
-        raise ValueError(f"{name}: cache records must be contiguous and "
-                         "4-byte aligned")
-    if slots is not None:
-        if slots.dtype not in (torch.int64, torch.int32) or slots.dim() != 1:
-            raise ValueError(f"{name}: slots must be 1-D int64 or int32, got "
-                             f"{slots.dtype} of {tuple(slots.shape)}")
-        if slots.device != cache.device:
-            raise ValueError(f"{name}: slots on {slots.device}, cache on "
-                             f"{cache.device}")
-
-
 def cache_write(cache: torch.Tensor, values: torch.Tensor,
                 slots: Optional[torch.Tensor] = None, fmt: str = "int8",
                 unique: bool = False) -> None:
@@ -221,28 +196,7 @@ def cache_write(cache: torch.Tensor, values: torch.Tensor,
     NaN throughout.  Slots outside the cache are padding and not written.
     Of several rows for one slot the last one is kept; ``unique=True``
     asserts that there are none (and saves the pass that finds out)."""
-    if values.dim() != 2 or values.dtype not in _VALUE_TYPES:
-        raise ValueError("cache_write: values must be 2-D float32, bfloat16 "
-                         f"or float16, got {values.dtype} of "
-                         f"{tuple(values.shape)}")
-    _check_records("cache_write", cache, values.shape[1], slots, fmt)
-    if values.device != cache.device:
-        raise ValueError(f"cache_write: values on {values.device}, cache on "
-                         f"{cache.device}")
-    n = cache.shape[0] if slots is None else slots.numel()
-    if values.shape[0] != n:
-        raise ValueError(f"cache_write: {values.shape[0]} rows of values for "
-                         f"{n} {'records' if slots is None else 'slots'}")
-    if cache.shape[0] > 1 and cache.stride(0) < cache.shape[1]:
-        raise ValueError("cache_write: cache records must not overlap")
-    if values.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("cache_write has no gradient: pass "
-                           "values.detach()")
-    if slots is not None:
-        slots = slots.contiguous()
     if _cuda(cache):
-        if values.stride(1) != 1:
-            values = values.contiguous()
         hip.ext().cache_write(cache, values, slots, fmt, unique)
         return
     reference.cache_write(cache, values, slots, fmt, unique)
@@ -254,15 +208,9 @@ def cache_read(cache: torch.Tensor, dim: int,
     """The values (n, ``dim``) of the records at ``slots``, or of all of them
     in order; ``dim`` and ``fmt`` as written.  A slot outside the cache is
     padding and reads as zeros."""
-    _check_records("cache_read", cache, int(dim), slots, fmt)
-    if dtype not in _VALUE_TYPES:
-        raise ValueError("cache_read: dtype must be float32, bfloat16 or "
-                         f"float16, got {dtype}")
-    if slots is not None:
-        slots = slots.contiguous()
     if _cuda(cache):
-        return hip.ext().cache_read(cache, int(dim), slots, fmt, dtype)
-    return reference.cache_read(cache, int(dim), slots, fmt, dtype)
+        return hip.ext().cache_read(cache, dim, slots, fmt, dtype)
+    return reference.cache_read(cache, dim, slots, fmt, dtype)
 
 
 # ---------------------------------------------------------------------------

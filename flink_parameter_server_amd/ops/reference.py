@@ -326,16 +326,56 @@ def sgns_step(vecs: torch.Tensor, center_slots: torch.Tensor,
 # match byte for byte.  A row with inf or NaN: NaN scale, zero codes.
 # ---------------------------------------------------------------------------
 
+_VALUE_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 _TINY = 2.0 ** -126
 _FP8_TOP = 240 * 2.0 ** 120  # the next code up stands for 2^128
 # the largest scale whose code 127 is finite (RN(FLT_MAX / 127) is one ulp up)
 _INT8_TOP = 2.6793883890187504e+36
 
 
+def _check_records(name: str, cache: torch.Tensor, dim: int,
+                   slots: Optional[torch.Tensor], fmt: str) -> None:
+    """What the HIP entry points refuse, refused alike."""
+    if fmt not in ("int8", "fp8"):
+        raise ValueError(f"{name}: unknown row format {fmt!r}")
+    if dim < 1 or cache.dtype != torch.uint8 or cache.dim() != 2 \
+            or cache.shape[1] != (dim + 3) // 4 * 4 + 4:
+        raise ValueError(
+            f"{name}: the cache of rows of {dim} values is uint8 of shape "
+            f"(rows, record_bytes({dim})), got {cache.dtype} of "
+            f"{tuple(cache.shape)}")
+    if cache.shape[0] and (cache.stride(1) != 1 or cache.stride(0) % 4
+                           or cache.data_ptr() % 4):
+        raise ValueError(f"{name}: cache records must be contiguous and "
+                         "4-byte aligned")
+    if slots is not None and (
+            slots.dtype not in (torch.int64, torch.int32) or slots.dim() != 1
+            or slots.device != cache.device):
+        raise ValueError(f"{name}: slots must be 1-D int64 or int32 on the "
+                         f"cache's device, got {slots.dtype} of "
+                         f"{tuple(slots.shape)} on {slots.device}")
+
+
 def cache_write(cache: torch.Tensor, values: torch.Tensor,
                 slots: Optional[torch.Tensor] = None, fmt: str = "int8",
                 unique: bool = False) -> None:
+    if values.dim() != 2 or values.dtype not in _VALUE_TYPES \
+            or values.device != cache.device:
+        raise ValueError("cache_write: values must be 2-D float32, bfloat16 "
+                         f"or float16 on the cache's device, got "
+                         f"{values.dtype} of {tuple(values.shape)} on "
+                         f"{values.device}")
     dim = values.shape[1]
+    _check_records("cache_write", cache, dim, slots, fmt)
+    n = cache.shape[0] if slots is None else slots.numel()
+    if values.shape[0] != n:
+        raise ValueError(f"cache_write: {values.shape[0]} rows of values for "
+                         f"{n} {'records' if slots is None else 'slots'}")
+    if cache.shape[0] > 1 and cache.stride(0) < cache.shape[1]:
+        raise ValueError("cache_write: cache records must not overlap")
+    if values.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("cache_write has no gradient: pass "
+                           "values.detach()")
     if not values.shape[0]:
         return
     x = values.detach().float()
@@ -378,6 +418,10 @@ def cache_write(cache: torch.Tensor, values: torch.Tensor,
 def cache_read(cache: torch.Tensor, dim: int,
                slots: Optional[torch.Tensor] = None, fmt: str = "int8",
                dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    _check_records("cache_read", cache, dim, slots, fmt)
+    if dtype not in _VALUE_TYPES:
+        raise ValueError("cache_read: dtype must be float32, bfloat16 or "
+                         f"float16, got {dtype}")
     rows = cache.shape[0]
     held = None
     if slots is not None:

@@ -22,7 +22,7 @@ setup(
             name="flink_parameter_server_amd._C",
             sources=["csrc/ps_kernels.hip", "csrc/row_cache.hip",
                      "csrc/muon.hip"],
-            depends=["csrc/ops.h"],
+            depends=["csrc/ops.h", "csrc/quads.h"],
             extra_compile_args={
                 "cxx": ["-O3"],
                 # no packed f32 arithmetic: some of its forms have given
