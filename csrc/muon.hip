@@ -20,11 +20,14 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
 #include "ops.h"
+#include "quads.h"
 
 namespace {
 
@@ -37,26 +40,6 @@ using half8 = __attribute__((ext_vector_type(8))) _Float16;
 using f32x4 = __attribute__((ext_vector_type(4))) float;
 using f64x4 = __attribute__((ext_vector_type(4))) double;
 
-template <typename T>
-__device__ inline float to_f32(T v);
-template <>
-__device__ inline float to_f32(float v) { return v; }
-template <>
-__device__ inline float to_f32(__half v) { return __half2float(v); }
-template <>
-__device__ inline float to_f32(__hip_bfloat16 v) { return __bfloat162float(v); }
-
-template <typename T>
-__device__ inline T from_f32(float v);
-template <>
-__device__ inline float from_f32(float v) { return v; }
-template <>
-__device__ inline __half from_f32(float v) { return __float2half_rn(v); }
-template <>
-__device__ inline __hip_bfloat16 from_f32(float v) {
-  return __float2bfloat16(v);
-}
-
 struct Coeffs { double a, b, c; };
 
 // What a product ends in: the values of `out` (T), or the weights' step
@@ -67,6 +50,11 @@ struct Result {
   bool step;
 };
 
+// The wave's number in a scalar register: branches on it cost nothing.
+__device__ inline int this_wave() {
+  return __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+}
+
 template <typename T>
 __device__ inline void finish(const Result& r, int64_t at, float o) {
   if (r.step) {
@@ -74,6 +62,23 @@ __device__ inline void finish(const Result& r, int64_t at, float o) {
     *w = *w * r.keep - r.rate * o;
   } else {
     ((T*)r.out)[at] = from_f32<T>(o);
+  }
+}
+
+// The same for four neighbours, `held` of them (any number).
+template <typename T>
+__device__ inline void finish_quad(const Result& r, int64_t at, float4 o,
+                                   int64_t held) {
+  if (r.step) {
+    float* w = (float*)r.out + at;
+    float4 v = load_quad(w, held);
+    v.x = v.x * r.keep - r.rate * o.x;
+    v.y = v.y * r.keep - r.rate * o.y;
+    v.z = v.z * r.keep - r.rate * o.z;
+    v.w = v.w * r.keep - r.rate * o.w;
+    store_quad(w, v, held);
+  } else {
+    store_quad((T*)r.out + at, o, held);
   }
 }
 
@@ -91,37 +96,68 @@ __device__ inline int64_t lower_bound(const int64_t* v, int64_t n,
   return lo;
 }
 
-__global__ __launch_bounds__(256) void k_touched(
-    int* __restrict__ touched, const int64_t* __restrict__ rows, int64_t n,
-    int64_t batch, int64_t m) {
-  int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (b >= batch) return;
-  int64_t lo = lower_bound(rows, n, b * m);
-  touched[b] = lo < n && rows[lo] < (b + 1) * m;
-}
-
-// M <- mu M + g and U = g + mu M (nesterov) or M, a wave a row.  g is the sum
-// of the row's gradients in the order of the push: rows are sorted, order[j]
-// is the place of the j-th in `grads`.
+// M <- mu M + g and U = g + mu M (nesterov) or M for `span` (at most 64) rows
+// of one matrix a block; touched[b] says for the kernels that follow whether
+// the push names a row of matrix b.  g is the sum of the row's gradients in
+// the order of the push: rows are sorted, order[j] is the place of the j-th
+// in `grads`.  Bound by memory: 16 bytes a value.
 __global__ __launch_bounds__(256) void k_momentum(
     float* __restrict__ u, float* __restrict__ momentum,
     const float* __restrict__ grads, const int64_t* __restrict__ rows,
-    const int64_t* __restrict__ order, const int* __restrict__ touched,
-    int64_t n, int64_t total, int64_t m, int64_t dim, float mu,
-    bool nesterov) {
-  const int lane = threadIdx.x % WAVE;
-  const int64_t waves = (int64_t)gridDim.x * (256 / WAVE);
-  for (int64_t r = (int64_t)blockIdx.x * (256 / WAVE) + threadIdx.x / WAVE;
-       r < total; r += waves) {
-    if (!touched[r / m]) continue;
-    const int64_t lo = lower_bound(rows, n, r);
-    for (int64_t c = lane; c < dim; c += WAVE) {
-      float g = 0.0f;
-      for (int64_t j = lo; j < n && rows[j] == r; ++j)
-        g += grads[(order ? order[j] : j) * dim + c];
-      float v = mu * momentum[r * dim + c] + g;
-      momentum[r * dim + c] = v;
-      u[r * dim + c] = nesterov ? g + mu * v : v;
+    const int64_t* __restrict__ order, int* __restrict__ touched, int64_t n,
+    int64_t m, int dim, int span, int group, float mu, bool nesterov) {
+  __shared__ int64_t first[64];
+  __shared__ int64_t ends[2];
+  const int64_t chunks = (m + span - 1) / span;
+  const int64_t b = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+  const int64_t r0 = b * m + chunk * span;
+  const int64_t count = min((int64_t)span, m - chunk * span);
+  if (threadIdx.x < 64) first[threadIdx.x] = -1;
+  if (threadIdx.x % WAVE == 0 && threadIdx.x < 2 * WAVE) {
+    // a push of every row has row r at place r
+    const int64_t x = threadIdx.x == 0 ? r0 : r0 + count;
+    const bool direct = x < n && rows[x] == x && (x == 0 || rows[x - 1] < x);
+    ends[threadIdx.x / WAVE] = direct ? x : lower_bound(rows, n, x);
+  }
+  __syncthreads();
+  const int64_t lo = ends[0], hi = ends[1];
+  bool some = hi > lo;
+  if (!some) {
+    int64_t at = lower_bound(rows, n, b * m);
+    some = at < n && rows[at] < (b + 1) * m;
+  }
+  if (chunk == 0 && threadIdx.x == 0) touched[b] = some;
+  if (!some) return;
+  for (int64_t j = lo + threadIdx.x; j < hi; j += 256)
+    if (j == lo || rows[j - 1] != rows[j]) first[rows[j] - r0] = j;
+  __syncthreads();
+  const int lane = threadIdx.x & (group - 1);
+  for (int r = threadIdx.x / group; r < count; r += 256 / group) {
+    const int64_t j0 = first[r], row = r0 + r;
+    for (int c = lane * 4; c < dim; c += group * 4) {
+      const int held = dim - c;
+      const int64_t at = row * dim + c;
+      float4 v = load_quad(momentum + at, held);
+      float4 g = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (j0 >= 0) {
+        g = load_quad(grads + (order ? order[j0] : j0) * dim + c, held);
+        for (int64_t j = j0 + 1; j < hi && rows[j] == row; ++j) {
+          float4 h = load_quad(grads + (order ? order[j] : j) * dim + c, held);
+          g.x += h.x;
+          g.y += h.y;
+          g.z += h.z;
+          g.w += h.w;
+        }
+      }
+      v.x = mu * v.x + g.x;
+      v.y = mu * v.y + g.y;
+      v.z = mu * v.z + g.z;
+      v.w = mu * v.w + g.w;
+      store_quad(momentum + at, v, held);
+      if (nesterov)
+        v = make_float4(g.x + mu * v.x, g.y + mu * v.y, g.z + mu * v.z,
+                        g.w + mu * v.w);
+      store_quad(u + at, v, held);
     }
   }
 }
@@ -131,30 +167,135 @@ __global__ __launch_bounds__(256) void k_momentum(
 // ---------------------------------------------------------------------
 
 constexpr int THIN_MAX = 320;  // the largest short side
+constexpr int NARROW = 64;     // up to here one block takes the whole chain
 constexpr int SUPER = 128;     // a block's square of G
 constexpr int KC = 32;         // long-axis places a block stages at a time
 constexpr int PITCH = SUPER + 16;
 
-// Partial sums of G over one chunk of the long axis: part[b][chunk][sp][sp],
-// tiles on and under the diagonal.  f64 matrix instructions: 16x16x4, a lane
-// holds row (or column) lane % 16 at place lane / 16.  They bound it: 64
-// cycles a tile and 4 places.
+// What the chain leaves for the product that applies it: X = ((u x) y), and P
+// stands in its planes as P / z.
+struct Norm { float x, y, z; };
+
+// X = U / n with n = |U|_F + eps as (u x) y: the power of two x keeps y and
+// the products normal for values near the ends of f32's range.  NaN for a
+// matrix that is not finite.
+__device__ inline double2 norm_factors(double sumsq, double eps) {
+  if (!(sumsq < INFINITY)) return make_double2(1.0, NAN);
+  const double n = sqrt(sumsq) + eps;
+  const double x = n > 0x1p60 ? 0x1p-60 : (n < 0x1p-60 ? 0x1p60 : 1.0);
+  return make_double2(x, 1.0 / (n * x));
+}
+
+__device__ inline void split(float v, _Float16& hi, _Float16& lo) {
+  hi = (_Float16)v;
+  lo = (_Float16)(v - (float)hi);
+}
+
+// The sum of a block's values, the same for every thread and run.
+__device__ inline double block_sum(double v, double* lds) {
+#pragma unroll
+  for (int o = WAVE / 2; o; o >>= 1) v += __shfl_xor(v, o);
+  __syncthreads();
+  if (threadIdx.x % WAVE == 0) lds[threadIdx.x / WAVE] = v;
+  __syncthreads();
+  v = 0;
+  for (int w = 0; w < (int)blockDim.x / WAVE; ++w) v += lds[w];
+  return v;
+}
+
+// Partial sums of G over one chunk of the long axis, short side up to
+// 16 NT <= 64: part[b][chunk][sp][sp], tiles on and under the diagonal.
+// f64 matrix instructions 16x16x4: a lane holds row (or column) lane % 16 at
+// place lane / 16; the order of the places is free, so four neighbouring ones
+// serve four instructions.  No LDS on the way: a wave reads its own places,
+// and four waves' sums are joined at the end.
+template <typename T, bool TALL, int NT>
+__global__ __launch_bounds__(256) void k_gram_narrow(
+    double* __restrict__ part, const T* __restrict__ u,
+    const int* __restrict__ touched, int64_t long_, int s, int64_t chunk) {
+  constexpr int SP = NT * 16, TILES = NT * (NT + 1) / 2;
+  __shared__ double lds[TILES * 256];
+  const int64_t b = blockIdx.y;
+  if (touched && !touched[b]) return;
+  const int lane = threadIdx.x % WAVE, wave = this_wave();
+  const T* x = u + b * long_ * s;
+  const int64_t k0 = blockIdx.x * chunk + wave * (chunk / 4);
+  const int64_t k1 = min(k0 + chunk / 4, long_);
+  f64x4 acc[TILES];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) acc[t] = (f64x4){0, 0, 0, 0};
+#pragma unroll 2
+  for (int64_t k = k0; k < k1; k += 16) {
+    float v[4][NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int col = t * 16 + lane % 16;
+      if (TALL) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int64_t kk = k + 4 * c + lane / 16;
+          v[c][t] = col < s && kk < k1 ? to_f32(x[kk * s + col]) : 0.0f;
+        }
+      } else {
+        const int64_t kk = k + lane / 16 * 4;
+        const float4 f = load_quad(x + col * long_ + kk,
+                                   col < s ? k1 - kk : 0);
+        v[0][t] = f.x;
+        v[1][t] = f.y;
+        v[2][t] = f.z;
+        v[3][t] = f.w;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j <= i; ++j)
+          acc[i * (i + 1) / 2 + j] = __builtin_amdgcn_mfma_f64_16x16x4f64(
+              v[c][i], v[c][j], acc[i * (i + 1) / 2 + j], 0, 0, 0);
+  }
+  for (int w = 0; w < 4; ++w) {
+    if (wave == w) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          double* to = lds + t * 256 + (lane / 16 + 4 * r) * 16 + lane % 16;
+          *to = w ? *to + acc[t][r] : acc[t][r];
+        }
+    }
+    __syncthreads();
+  }
+  double* out = part + (b * gridDim.x + blockIdx.x) * (int64_t)SP * SP;
+  int ti = 0, tj = 0;
+  for (int t = 0; t < TILES; ++t) {
+    out[(ti * 16 + threadIdx.x / 16) * SP + tj * 16 + threadIdx.x % 16] =
+        lds[t * 256 + threadIdx.x];
+    if (++tj > ti) { tj = 0; ++ti; }
+  }
+}
+
+// The same for short sides up to THIN_MAX: a block takes the places of one
+// chunk for a SUPER x SUPER square of G, through LDS.  The matrix
+// instructions bound it: 64 cycles a tile and 4 places.
 template <typename T, bool TALL>
 __global__ __launch_bounds__(256) void k_gram64(
-    double* __restrict__ part, const T* __restrict__ u,
-    const int* __restrict__ touched, int64_t long_, int s, int sp,
-    int64_t chunk) {
+    double* __restrict__ part, double* __restrict__ traces,
+    const T* __restrict__ u, const int* __restrict__ touched, int64_t long_,
+    int s, int sp, int64_t chunk) {
   __shared__ float rows_[KC][PITCH], cols_[KC][PITCH];
+  __shared__ double sums[4];
   const int64_t b = blockIdx.z;
   if (touched && !touched[b]) return;
   // blockIdx.y counts the pairs of super-tiles (si >= sj)
   int si = 0, sj = blockIdx.y;
   while (sj > si) { sj -= si + 1; ++si; }
   const bool diagonal = si == sj;
-  const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+  const int lane = threadIdx.x % WAVE, wave = this_wave();
   const T* x = u + b * long_ * s;
   const int64_t k0 = blockIdx.x * chunk;
-  const int64_t k1 = k0 + chunk < long_ ? k0 + chunk : long_;
+  const int64_t k1 = min(k0 + chunk, long_);
   const int pair[2] = {wave, 7 - wave};  // this wave's rows of tiles
 
   f64x4 acc[2][8];
@@ -163,24 +304,50 @@ __global__ __launch_bounds__(256) void k_gram64(
 #pragma unroll
     for (int t = 0; t < 8; ++t) acc[p][t] = (f64x4){0, 0, 0, 0};
 
-  auto stage = [&](float (*to)[PITCH], int base, int64_t k) {
-    for (int e = threadIdx.x; e < KC * SUPER; e += 256) {
-      // neighbours in memory are neighbours in threads
-      int kk = TALL ? e / SUPER : e % KC, c = TALL ? e % SUPER : e / KC;
-      int col = base + c;
-      float v = 0.0f;
-      if (col < s && k + kk < k1)
-        v = to_f32(TALL ? x[(k + kk) * s + col] : x[col * long_ + k + kk]);
-      to[kk][c] = v;
+  // four quads a thread: along the columns (TALL) or along the places
+  float4 next[2][4];
+  auto fetch = [&](int o, int base, int64_t k) {
+#pragma unroll
+    for (int l = 0; l < 4; ++l) {
+      const int e = threadIdx.x + l * 256;
+      const int kk = TALL ? e / 32 : e % 8 * 4, c = TALL ? e % 32 * 4 : e / 8;
+      const int64_t held = TALL ? (k + kk < k1 ? s - base - c : 0)
+                                : (base + c < s ? k1 - k - kk : 0);
+      next[o][l] = load_quad(TALL ? x + (k + kk) * s + base + c
+                                  : x + (int64_t)(base + c) * long_ + k + kk,
+                             held);
+    }
+  };
+  auto put = [&](float (*to)[PITCH], int o) {
+#pragma unroll
+    for (int l = 0; l < 4; ++l) {
+      const int e = threadIdx.x + l * 256;
+      const float4 f = next[o][l];
+      if (TALL) {
+        *(float4*)&to[e / 32][e % 32 * 4] = f;
+      } else {
+        const int kk = e % 8 * 4, c = e / 8;
+        to[kk][c] = f.x;
+        to[kk + 1][c] = f.y;
+        to[kk + 2][c] = f.z;
+        to[kk + 3][c] = f.w;
+      }
     }
   };
 
+  fetch(0, si * SUPER, k0);
+  if (!diagonal) fetch(1, sj * SUPER, k0);
   for (int64_t k = k0; k < k1; k += KC) {
     __syncthreads();
-    stage(rows_, si * SUPER, k);
-    if (!diagonal) stage(cols_, sj * SUPER, k);
+    put(rows_, 0);
+    if (!diagonal) put(cols_, 1);
     __syncthreads();
+    if (k + KC < k1) {
+      fetch(0, si * SUPER, k + KC);
+      if (!diagonal) fetch(1, sj * SUPER, k + KC);
+    }
     const float (*cols)[PITCH] = diagonal ? rows_ : cols_;
+#pragma unroll 2
     for (int q = 0; q < KC; q += 4) {
       const int kk = q + lane / 16;
       double av[2];
@@ -200,6 +367,7 @@ __global__ __launch_bounds__(256) void k_gram64(
     }
   }
   double* out = part + (b * gridDim.x + blockIdx.x) * (int64_t)sp * sp;
+  double trace = 0;
 #pragma unroll
   for (int p = 0; p < 2; ++p)
 #pragma unroll
@@ -207,147 +375,356 @@ __global__ __launch_bounds__(256) void k_gram64(
       int i0 = si * SUPER + pair[p] * 16, j0 = sj * SUPER + t * 16;
       if ((diagonal && t > pair[p]) || i0 >= sp || j0 >= sp) continue;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        out[(int64_t)(i0 + lane / 16 + 4 * r) * sp + j0 + lane % 16] =
-            acc[p][t][r];
+      for (int r = 0; r < 4; ++r) {
+        int i = i0 + lane / 16 + 4 * r, j = j0 + lane % 16;
+        out[(int64_t)i * sp + j] = acc[p][t][r];
+        if (i == j) trace += acc[p][t][r];
+      }
     }
+  if (diagonal) {
+    trace = block_sum(trace, sums);
+    if (threadIdx.x == 0)
+      traces[(b * gridDim.x + blockIdx.x) * ((sp + SUPER - 1) / SUPER) + si] =
+          trace;
+  }
 }
 
-// G = the sum of the parts, in their order; the upper half by symmetry.
+// G = nu^2 times the sum of the parts, in their order; the upper half by
+// symmetry.  nu from the trace, |U|_F^2.
 __global__ __launch_bounds__(256) void k_gram_sum(
-    double* __restrict__ g, const double* __restrict__ part,
-    const int* __restrict__ touched, int chunks, int sp) {
+    double* __restrict__ g, Norm* __restrict__ norm,
+    const double* __restrict__ part, const double* __restrict__ traces,
+    const int* __restrict__ touched, int chunks, int sp, double eps) {
+  __shared__ double sums[4];
   const int64_t b = blockIdx.y;
   if (touched && !touched[b]) return;
+  const int count = chunks * ((sp + SUPER - 1) / SUPER);
+  double t = 0;
+  for (int k = threadIdx.x; k < count; k += 256) t += traces[b * count + k];
+  const double2 f = norm_factors(block_sum(t, sums), eps);
+  const double nu = f.x * f.y;
+  if (blockIdx.x == 0 && threadIdx.x == 0)
+    norm[b] = Norm{(float)f.x, (float)f.y, 0.0f};
   const int64_t size = (int64_t)sp * sp;
   int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (e >= size) return;
   int i = e / sp, j = e % sp;
   if (i < j) return;
   const double* p = part + b * chunks * size + e;
-  double sum = 0;
-  for (int k = 0; k < chunks; ++k) sum += p[k * size];
-  g[b * size + e] = sum;
-  g[b * size + (int64_t)j * sp + i] = sum;
+  double sum[4] = {0, 0, 0, 0};
+  int k = 0;
+  for (; k + 4 <= chunks; k += 4)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sum[q] += p[(k + q) * size];
+  for (; k < chunks; ++k) sum[0] += p[k * size];
+  const double v = ((sum[0] + sum[1]) + (sum[2] + sum[3])) * nu * nu;
+  g[b * size + e] = v;
+  g[b * size + (int64_t)j * sp + i] = v;
 }
 
-// X = U / n with n = |U|_F + eps as (u x) y: the power of two x keeps y and
-// the products normal for values near the ends of f32's range.  NaN for a
-// matrix that is not finite.
-__device__ inline double2 norm_factors(double sumsq, double eps) {
-  if (!(sumsq < INFINITY)) return make_double2(1.0, NAN);
-  const double n = sqrt(sumsq) + eps;
-  const double x = n > 0x1p60 ? 0x1p-60 : (n < 0x1p-60 ? 0x1p60 : 1.0);
-  return make_double2(x, 1.0 / (n * x));
-}
+// One product of commuting symmetric matrices (so it is symmetric too):
+// out = x y, or, if `poly`, a I + b x + c (x y).
+struct SmallMul {
+  double* out;
+  const double *x, *y;
+  bool poly;
+};
 
-// |U|_F^2 is G's trace; G becomes X's.  One block a matrix.
-__global__ __launch_bounds__(256) void k_gram_norm(
-    double* __restrict__ g, double2* __restrict__ nu,
-    const int* __restrict__ touched, int sp, double eps) {
-  __shared__ double lds[256];
-  const int64_t b = blockIdx.x;
-  if (touched && !touched[b]) return;
-  double* m = g + b * (int64_t)sp * sp;
-  double t = 0;
-  for (int i = threadIdx.x; i < sp; i += 256) t += m[(int64_t)i * sp + i];
-  lds[threadIdx.x] = t;
-  __syncthreads();
-  for (int o = 128; o; o >>= 1) {
-    if (threadIdx.x < o) lds[threadIdx.x] += lds[threadIdx.x + o];
-    __syncthreads();
-  }
-  const double2 f = norm_factors(lds[0], eps);
-  const double v = f.x * f.y;
-  if (threadIdx.x == 0) nu[b] = f;
-  for (int64_t e = threadIdx.x; e < (int64_t)sp * sp; e += 256) m[e] *= v * v;
-}
-
-// out = x y for commuting symmetric matrices (so out is symmetric): a wave a
-// tile on or under the diagonal, mirrored.  q, if given, becomes
-// a I + b x + c out (used with y = x).
-__global__ __launch_bounds__(64) void k_small_mul(
-    double* __restrict__ out, double* __restrict__ q,
-    const double* __restrict__ x, const double* __restrict__ y,
-    const int* __restrict__ touched, int s, int sp, Coeffs k) {
+// A block a tile on or under the diagonal, mirrored; the four waves share the
+// places of the sum.  blockIdx.z counts the products.
+__global__ __launch_bounds__(256) void k_small_mul(
+    SmallMul j0, SmallMul j1, const int* __restrict__ touched, int s, int sp,
+    Coeffs k) {
+  __shared__ double lds[4][256];
   const int64_t b = blockIdx.y;
   if (touched && !touched[b]) return;
+  const SmallMul job = blockIdx.z ? j1 : j0;
   int ti = 0, tj = blockIdx.x;
   while (tj > ti) { tj -= ti + 1; ++ti; }
   const int64_t base = b * (int64_t)sp * sp;
-  const int lane = threadIdx.x;
-  const double* xr = x + base + (int64_t)(ti * 16 + lane % 16) * sp;
-  const double* yr = y + base + (int64_t)(tj * 16 + lane % 16) * sp;
+  const int lane = threadIdx.x % WAVE, wave = this_wave();
+  const double* xr = job.x + base + (int64_t)(ti * 16 + lane % 16) * sp;
+  const double* yr = job.y + base + (int64_t)(tj * 16 + lane % 16) * sp;
   f64x4 acc = (f64x4){0, 0, 0, 0};
-  for (int kk = lane / 16; kk < sp; kk += 4)
-    acc = __builtin_amdgcn_mfma_f64_16x16x4f64(xr[kk], yr[kk], acc, 0, 0, 0);
+#pragma unroll 2
+  for (int kk = wave * 16; kk < sp; kk += 64) {
+    const f64x4 xv = *(const f64x4*)(xr + kk + lane / 16 * 4);
+    const f64x4 yv = *(const f64x4*)(yr + kk + lane / 16 * 4);
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    int i = ti * 16 + lane / 16 + 4 * r, j = tj * 16 + lane % 16;
-    if (i < j) continue;  // a tile on the diagonal
-    int64_t at = base + (int64_t)i * sp + j, ta = base + (int64_t)j * sp + i;
-    if (q) {
-      double v = k.b * x[at] + k.c * acc[r] + (i == j && i < s ? k.a : 0.0);
-      q[at] = v;
-      q[ta] = v;
-    } else {
-      out[at] = acc[r];
-      out[ta] = acc[r];
+    for (int c = 0; c < 4; ++c)
+      acc = __builtin_amdgcn_mfma_f64_16x16x4f64(xv[c], yv[c], acc, 0, 0, 0);
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    lds[wave][(lane / 16 + 4 * r) * 16 + lane % 16] = acc[r];
+  __syncthreads();
+  const int e = threadIdx.x;
+  double v = (lds[0][e] + lds[1][e]) + (lds[2][e] + lds[3][e]);
+  const int i = ti * 16 + e / 16, j = tj * 16 + e % 16;
+  if (i < j) return;  // a tile on the diagonal
+  const int64_t at = base + (int64_t)i * sp + j, ta = base + (int64_t)j * sp + i;
+  if (job.poly) v = k.b * job.x[at] + k.c * v + (i == j && i < s ? k.a : 0.0);
+  job.out[at] = v;
+  job.out[ta] = v;
+}
+
+// P into two f16 planes of jp x kp places (zeros around it), scaled by a power
+// of two that takes its largest value to 2^12.  The block's threads together;
+// p(i, j) reads P.
+template <typename P>
+__device__ inline void put_planes(_Float16* planes, int64_t plane, int jp,
+                                  int kp, int s, P p, Norm* norm,
+                                  double* lds) {
+  double top = 0;
+  for (int e = threadIdx.x; e < s * s; e += blockDim.x)
+    top = fmax(top, fabs(p(e / s, e % s)));
+#pragma unroll
+  for (int o = WAVE / 2; o; o >>= 1) top = fmax(top, __shfl_xor(top, o));
+  __syncthreads();
+  if (threadIdx.x % WAVE == 0) lds[threadIdx.x / WAVE] = top;
+  __syncthreads();
+  for (int w = 0; w < (int)blockDim.x / WAVE; ++w) top = fmax(top, lds[w]);
+  const int e2 = top > 0 && top < INFINITY ? 12 - ilogb(top) : 0;
+  for (int e = threadIdx.x; e < jp * kp; e += blockDim.x) {
+    const int i = e / kp, j = e % kp;
+    const float v = i < s && j < s ? (float)ldexp(p(i, j), e2) : 0.0f;
+    split(v, planes[e], planes[plane + e]);
+  }
+  if (threadIdx.x == 0) norm->z = (float)ldexp(1.0, -e2);
+}
+
+__global__ __launch_bounds__(1024) void k_small_out(
+    _Float16* __restrict__ planes, const double* __restrict__ p,
+    Norm* __restrict__ norm, const int* __restrict__ touched, int s, int sp,
+    int jp, int kp) {
+  __shared__ double lds[16];
+  const int64_t b = blockIdx.x;
+  if (touched && !touched[b]) return;
+  const double* at = p + b * (int64_t)sp * sp;
+  put_planes(planes + b * (int64_t)jp * kp, gridDim.x * (int64_t)jp * kp, jp,
+             kp, s, [&](int i, int j) { return at[i * sp + j]; }, norm + b,
+             lds);
+}
+
+// The chain for short sides up to 64: one block a matrix, G, Q, P and G Q in
+// LDS; a wave takes every fourth tile on or under the diagonal.
+template <int NT>
+__global__ __launch_bounds__(256) void k_chain(
+    _Float16* __restrict__ planes, Norm* __restrict__ norm,
+    const double* __restrict__ part, const int* __restrict__ touched,
+    int chunks, int s, int steps, Coeffs k, double eps, int jp, int kp) {
+  constexpr int SP = NT * 16, LP = SP + 2, TILES = NT * (NT + 1) / 2;
+  constexpr int MINE = (TILES + 3) / 4;
+  __shared__ double g[SP * LP], q[SP * LP], p[SP * LP], t[SP * LP], sums[4];
+  const int64_t b = blockIdx.x;
+  if (touched && !touched[b]) return;
+  const int lane = threadIdx.x % WAVE, wave = this_wave();
+  const double* from = part + b * chunks * (int64_t)SP * SP;
+  double trace = 0;
+  for (int e = threadIdx.x; e < SP * SP; e += 256) {
+    const int i = e / SP, j = e % SP;
+    if (i < j) continue;
+    double sum[4] = {0, 0, 0, 0};
+    int c = 0;
+    for (; c + 4 <= chunks; c += 4)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) sum[w] += from[(int64_t)(c + w) * SP * SP + e];
+    for (; c < chunks; ++c) sum[0] += from[(int64_t)c * SP * SP + e];
+    const double v = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    g[i * LP + j] = v;
+    g[j * LP + i] = v;
+    if (i == j) trace += v;
+  }
+  const double2 f = norm_factors(block_sum(trace, sums), eps);
+  const double nu = f.x * f.y;
+  if (threadIdx.x == 0) norm[b] = Norm{(float)f.x, (float)f.y, 0.0f};
+  for (int e = threadIdx.x; e < SP * LP; e += 256)
+    if (e % LP < SP) g[e] *= nu * nu;
+  __syncthreads();
+
+  int ti[MINE], tj[MINE];
+#pragma unroll
+  for (int o = 0; o < MINE; ++o) {
+    ti[o] = 0;
+    tj[o] = wave + o * 4;
+    while (tj[o] > ti[o]) { tj[o] -= ti[o] + 1; ++ti[o]; }
+  }
+  // out = x y, or a I + b x + c x y; `out` may be one of the operands
+  auto mul = [&](double* out, const double* x, const double* y, bool poly) {
+    f64x4 acc[MINE];
+#pragma unroll
+    for (int o = 0; o < MINE; ++o) {
+      acc[o] = (f64x4){0, 0, 0, 0};
+      if (ti[o] >= NT) continue;
+      const double* xr = x + (ti[o] * 16 + lane % 16) * LP + lane / 16;
+      const double* yr = y + (tj[o] * 16 + lane % 16) * LP + lane / 16;
+#pragma unroll 4
+      for (int kk = 0; kk < SP; kk += 4)
+        acc[o] = __builtin_amdgcn_mfma_f64_16x16x4f64(xr[kk], yr[kk], acc[o],
+                                                      0, 0, 0);
+      if (poly) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = ti[o] * 16 + lane / 16 + 4 * r;
+          const int j = tj[o] * 16 + lane % 16;
+          acc[o][r] = k.b * x[i * LP + j] + k.c * acc[o][r] +
+                      (i == j && i < s ? k.a : 0.0);
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int o = 0; o < MINE; ++o) {
+      if (ti[o] >= NT) continue;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = ti[o] * 16 + lane / 16 + 4 * r;
+        const int j = tj[o] * 16 + lane % 16;
+        if (i < j) continue;
+        out[i * LP + j] = acc[o][r];
+        out[j * LP + i] = acc[o][r];
+      }
+    }
+    __syncthreads();
+  };
+  for (int step = 0; step < steps; ++step) {
+    double* qi = step ? q : p;  // the first Q is P
+    mul(qi, g, g, true);
+    if (step) mul(p, p, q, false);
+    if (step + 1 < steps) {
+      mul(t, g, qi, false);
+      mul(g, qi, t, false);
     }
   }
+  put_planes(planes + b * (int64_t)jp * kp, gridDim.x * (int64_t)jp * kp, jp,
+             kp, s, [&](int i, int j) { return p[i * LP + j]; }, norm + b,
+             sums);
 }
 
-// P with the norm's second factor, in f32
-__global__ __launch_bounds__(256) void k_small_out(
-    float* __restrict__ pf, const double* __restrict__ p,
-    const double2* __restrict__ nu, const int* __restrict__ touched, int sp) {
-  const int64_t b = blockIdx.y;
-  if (touched && !touched[b]) return;
-  int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e < (int64_t)sp * sp)
-    pf[b * (int64_t)sp * sp + e] = (float)(p[b * (int64_t)sp * sp + e] *
-                                           nu[b].y);
-}
-
-// O = U P (TALL) or P U: a wave 16 places of the long axis by 64 of the short
-// one, f32 matrix instructions 16x16x4.
-template <typename T, bool TALL>
+// O = U P (TALL) or P U: P in LDS, 16 JT places of the short side and KS
+// places of the sum at a time; a wave 32 places of the long axis a turn, whose
+// values it takes from memory to the matrix instructions by itself, split in
+// two planes on the way.  Bound by memory.
+template <typename T, bool TALL, int JT, int KS>
 __global__ __launch_bounds__(256) void k_thin_apply(
-    Result res, const T* __restrict__ u, const float* __restrict__ pf,
-    const double2* __restrict__ nu, const int* __restrict__ touched,
-    int64_t long_, int s, int sp) {
+    Result res, const T* __restrict__ u, const _Float16* __restrict__ planes,
+    const Norm* __restrict__ norm, const int* __restrict__ touched,
+    int64_t long_, int s, int jp, int kp) {
+  constexpr int LP = KS + 8;  // rows of eight lanes' pieces in other banks
+  __shared__ _Float16 lds[2][JT * 16 * LP];
   const int64_t b = blockIdx.z;
   if (touched && !touched[b]) return;
-  const float pre = (float)nu[b].x;
-  const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
-  const int64_t r = ((int64_t)blockIdx.x * 4 + wave) * 16 + lane % 16;
-  const int j0 = blockIdx.y * 64;
+  const int lane = threadIdx.x % WAVE, wave = this_wave();
+  const int j0 = blockIdx.y * JT * 16;
+  const Norm nm = norm[b];
+  const float up = nm.y * UP, down = nm.z / UP;
   const T* x = u + b * long_ * s;
-  const float* p = pf + b * (int64_t)sp * sp;
-  f32x4 acc[4];
+  const _Float16* p = planes + (b * jp + j0) * (int64_t)kp;
+  const int64_t plane = gridDim.z * (int64_t)jp * kp;
+  const int kchunks = (kp + KS - 1) / KS;
+
+  auto stage = [&](int kc) {
+    __syncthreads();
+    for (int e = threadIdx.x; e < 2 * JT * 16 * (KS / 8); e += 256) {
+      const int h = e / (JT * 16 * (KS / 8)), r = e / (KS / 8) % (JT * 16);
+      const int c = e % (KS / 8) * 8;
+      half8 v = {};
+      if (kc + c < kp)
+        v = *(const half8*)(p + h * plane + (int64_t)r * kp + kc + c);
+      *(half8*)&lds[h][r * LP + c] = v;
+    }
+    __syncthreads();
+  };
+  if (kchunks == 1) stage(0);
+
+  for (int64_t base = (int64_t)blockIdx.x * 128; base < long_;
+       base += (int64_t)gridDim.x * 128) {
+    f32x4 acc[JT][2];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) acc[t] = (f32x4){0, 0, 0, 0};
-  for (int k = lane / 16; k < sp; k += 4) {
-    float v = 0.0f;
-    if (k < s && r < long_) v = to_f32(TALL ? x[r * s + k] : x[k * long_ + r]) * pre;
+    for (int t = 0; t < JT; ++t)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      int j = j0 + t * 16 + lane % 16;
-      float w = j < sp ? p[(int64_t)k * sp + j] : 0.0f;
-      // D[short][long]
-      acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, v, acc[t], 0, 0, 0);
+      for (int w = 0; w < 2; ++w) acc[t][w] = (f32x4){0, 0, 0, 0};
+    const int64_t r0 = base + wave * 32 + lane % 16;
+    for (int kc = 0; kc < kp; kc += KS) {
+      if (kchunks > 1) stage(kc);
+      float raw[KS / 32][2][8];
+#pragma unroll
+      for (int ks = 0; ks < KS / 32; ++ks)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const int64_t r = r0 + w * 16;
+          const int k = kc + ks * 32 + lane / 16 * 8;
+          if (TALL) {
+            const int held = r < long_ ? s - k : 0;
+            const float4 f = load_quad(x + r * s + k, held);
+            const float4 g = load_quad(x + r * s + k + 4, held - 4);
+            raw[ks][w][0] = f.x;
+            raw[ks][w][1] = f.y;
+            raw[ks][w][2] = f.z;
+            raw[ks][w][3] = f.w;
+            raw[ks][w][4] = g.x;
+            raw[ks][w][5] = g.y;
+            raw[ks][w][6] = g.z;
+            raw[ks][w][7] = g.w;
+          } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              raw[ks][w][c] = r < long_ && k + c < s
+                                  ? to_f32(x[(int64_t)(k + c) * long_ + r])
+                                  : 0.0f;
+          }
+        }
+#pragma unroll
+      for (int ks = 0; ks < KS / 32; ++ks) {
+        half8 hi[2], lo[2];
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            _Float16 h, l;
+            split(raw[ks][w][c] * nm.x * up, h, l);
+            hi[w][c] = h;
+            lo[w][c] = l;
+          }
+#pragma unroll
+        for (int t = 0; t < JT; ++t) {
+          const int at = (t * 16 + lane % 16) * LP + ks * 32 + lane / 16 * 8;
+          const half8 ph = *(const half8*)&lds[0][at];
+          const half8 pl = *(const half8*)&lds[1][at];
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            acc[t][w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                pl, hi[w], acc[t][w], 0, 0, 0);
+            acc[t][w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                ph, lo[w], acc[t][w], 0, 0, 0);
+            acc[t][w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                ph, hi[w], acc[t][w], 0, 0, 0);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const int64_t r = r0 + w * 16;
+      if (r >= long_) continue;
+#pragma unroll
+      for (int t = 0; t < JT; ++t) {
+        const int j = j0 + t * 16 + lane / 16 * 4;
+        const float4 o = make_float4(acc[t][w][0] * down, acc[t][w][1] * down,
+                                     acc[t][w][2] * down, acc[t][w][3] * down);
+        if (TALL) {
+          finish_quad<T>(res, b * long_ * s + r * s + j, o, s - j);
+        } else {
+          const float v[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (j + i < s)
+              finish<T>(res, b * long_ * s + (int64_t)(j + i) * long_ + r,
+                        v[i]);
+        }
+      }
     }
   }
-  if (r >= long_) return;
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      int j = j0 + t * 16 + (lane / 16) * 4 + i;
-      if (j < s)
-        finish<T>(res, b * long_ * s + (TALL ? r * s + j : j * long_ + r),
-                  acc[t][i]);
-    }
 }
 
 // ---------------------------------------------------------------------
@@ -359,11 +736,6 @@ struct Planes {
   _Float16* p;
   int64_t plane, pitch, batch;  // batch: from one matrix to the next
 };
-
-__device__ inline void split(float v, _Float16& hi, _Float16& lo) {
-  hi = (_Float16)v;
-  lo = (_Float16)(v - (float)hi);
-}
 
 template <typename T>
 __global__ __launch_bounds__(256) void k_sumsq(
@@ -458,7 +830,7 @@ __global__ __launch_bounds__(256) void k_product(
     bi = 0;
     while (bj > bi) { bj -= bi + 1; ++bi; }
   }
-  const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+  const int lane = threadIdx.x % WAVE, wave = this_wave();
   const int wi = wave / 2 * (NT / 2), wj = wave % 2 * (NT / 2);
 
   const _Float16* src[2] = {
@@ -589,54 +961,85 @@ template <typename T, bool TALL>
 void run_thin(const Chain& c) {
   const int s = std::min(c.m, c.n);
   const int64_t long_ = std::max(c.m, c.n);
-  const int sp = round_up(s, 16), nt = sp / 16;
+  const bool narrow = s <= NARROW;
+  const int nt = !narrow ? (s + 15) / 16 : s <= 16 ? 1 : s <= 32 ? 2 : 4;
+  const int sp = nt * 16;
   const int super = (s + SUPER - 1) / SUPER, pairs = super * (super + 1) / 2;
-  // chunks of 256 places at least, about two blocks a CU
-  int64_t chunks = std::min<int64_t>((long_ + 255) / 256,
-                                     std::max<int64_t>(1, 512 / (c.batch *
-                                                                 pairs)));
-  const int64_t chunk = round_up((long_ + chunks - 1) / chunks, KC);
+  // chunks: about two blocks a CU, of at least 64 places (16 a wave) or KC
+  const int64_t least = narrow ? 64 : KC;
+  int64_t chunks = std::min<int64_t>(
+      (long_ + least - 1) / least,
+      std::max<int64_t>(1, 512 / (c.batch * (narrow ? 1 : pairs))));
+  const int64_t chunk = round_up((long_ + chunks - 1) / chunks, least);
   chunks = (long_ + chunk - 1) / chunk;
   const int64_t size = (int64_t)sp * sp;
+  // the planes of P: JT * 16 rows a block, KS places of the sum
+  const int jt = s <= 32 ? 2 : s <= 64 ? 4 : 8;
+  const int jp = round_up(s, jt * 16), kp = round_up(s, 32);
   auto f64 = c.options.dtype(at::kDouble);
   auto part = at::empty({c.batch * chunks * size}, f64);
-  auto work = at::empty({6, c.batch * size}, f64);
-  auto nu = at::empty({2 * c.batch}, f64);
-  double2* nus = (double2*)nu.data_ptr<double>();
-  auto pf = at::empty({c.batch * size}, c.options.dtype(at::kFloat));
-  double* w[6];
-  for (int i = 0; i < 6; ++i) w[i] = work.data_ptr<double>() + i * c.batch * size;
-  hipLaunchKernelGGL((k_gram64<T, TALL>), dim3(chunks, pairs, c.batch),
-                     dim3(256), 0, c.stream, part.data_ptr<double>(),
-                     (const T*)c.u, c.touched, long_, s, sp, chunk);
-  const dim3 all((size + 255) / 256, c.batch);
-  double *g = w[0], *q = w[1], *p = w[2], *t = w[3], *g2 = w[4], *p2 = w[5];
-  hipLaunchKernelGGL(k_gram_sum, all, dim3(256), 0, c.stream, g,
-                     part.data_ptr<double>(), c.touched, (int)chunks, sp);
-  hipLaunchKernelGGL(k_gram_norm, dim3(c.batch), dim3(256), 0, c.stream, g,
-                     nus, c.touched, sp, c.eps);
-  const dim3 tiles(nt * (nt + 1) / 2, c.batch);
-  auto mul = [&](double* out, double* poly, const double* x, const double* y) {
-    hipLaunchKernelGGL(k_small_mul, tiles, dim3(64), 0, c.stream, out, poly, x,
-                       y, c.touched, s, sp, c.k);
-  };
-  for (int i = 0; i < c.steps; ++i) {
-    // Q from G; P <- P Q (the first P is Q); G <- Q (G Q)
-    double* qi = i == 0 ? p : q;
-    mul(nullptr, qi, g, g);
-    if (i > 0) { mul(p2, nullptr, p, q); std::swap(p, p2); }
-    if (i + 1 < c.steps) {
-      mul(t, nullptr, g, qi);
-      mul(g2, nullptr, qi, t);
-      std::swap(g, g2);
+  auto pl = at::empty({2 * c.batch * jp * kp}, c.options.dtype(at::kHalf));
+  auto nm = at::empty({c.batch * 3}, c.options.dtype(at::kFloat));
+  _Float16* planes = (_Float16*)pl.data_ptr();
+  Norm* norm = (Norm*)nm.data_ptr();
+  double* parts = part.data_ptr<double>();
+  if (narrow) {
+    auto go = [&](auto* gram, auto* chain) {
+      hipLaunchKernelGGL(gram, dim3(chunks, c.batch), dim3(256), 0, c.stream,
+                         parts, (const T*)c.u, c.touched, long_, s, chunk);
+      hipLaunchKernelGGL(chain, dim3(c.batch), dim3(256), 0, c.stream, planes,
+                         norm, parts, c.touched, (int)chunks, s, c.steps, c.k,
+                         c.eps, jp, kp);
+    };
+    if (nt == 1) go(k_gram_narrow<T, TALL, 1>, k_chain<1>);
+    else if (nt == 2) go(k_gram_narrow<T, TALL, 2>, k_chain<2>);
+    else go(k_gram_narrow<T, TALL, 4>, k_chain<4>);
+  } else {
+    auto tr = at::empty({c.batch * chunks * super}, f64);
+    auto work = at::empty({6, c.batch * size}, f64);
+    double* w[6];
+    for (int i = 0; i < 6; ++i)
+      w[i] = work.data_ptr<double>() + i * c.batch * size;
+    hipLaunchKernelGGL((k_gram64<T, TALL>), dim3(chunks, pairs, c.batch),
+                       dim3(256), 0, c.stream, parts, tr.data_ptr<double>(),
+                       (const T*)c.u, c.touched, long_, s, sp, chunk);
+    double *g = w[0], *q = w[1], *p = w[2], *t = w[3], *g2 = w[4], *p2 = w[5];
+    hipLaunchKernelGGL(k_gram_sum, dim3((size + 255) / 256, c.batch),
+                       dim3(256), 0, c.stream, g, norm, parts,
+                       tr.data_ptr<double>(), c.touched, (int)chunks, sp,
+                       c.eps);
+    auto mul = [&](SmallMul j0, SmallMul j1, int jobs) {
+      hipLaunchKernelGGL(k_small_mul, dim3(nt * (nt + 1) / 2, c.batch, jobs),
+                         dim3(256), 0, c.stream, j0, j1, c.touched, s, sp,
+                         c.k);
+    };
+    for (int i = 0; i < c.steps; ++i) {
+      // Q from G; P <- P Q (the first P is Q); G <- Q (G Q)
+      const bool last = i + 1 == c.steps;
+      double* qi = i == 0 ? p : q;
+      mul({qi, g, g, true}, {}, 1);
+      if (i == 0 && !last) mul({t, g, qi, false}, {}, 1);
+      if (i > 0) mul({p2, p, q, false}, {t, g, qi, false}, last ? 1 : 2);
+      if (!last) {
+        mul({g2, qi, t, false}, {}, 1);
+        std::swap(g, g2);
+      }
+      if (i > 0) std::swap(p, p2);
     }
+    hipLaunchKernelGGL(k_small_out, dim3(c.batch), dim3(1024), 0, c.stream,
+                       planes, p, norm, c.touched, s, sp, jp, kp);
   }
-  hipLaunchKernelGGL(k_small_out, all, dim3(256), 0, c.stream,
-                     pf.data_ptr<float>(), p, nus, c.touched, sp);
-  hipLaunchKernelGGL((k_thin_apply<T, TALL>),
-                     dim3((long_ + 63) / 64, (s + 63) / 64, c.batch),
-                     dim3(256), 0, c.stream, c.res, (const T*)c.u,
-                     pf.data_ptr<float>(), nus, c.touched, long_, s, sp);
+  // turns of 128 places; a few a block where P's planes come in once
+  const int64_t turns = (long_ + 127) / 128;
+  const dim3 grid(std::min<int64_t>(turns, 2048), jp / (jt * 16), c.batch);
+  auto apply = [&](auto* kfn) {
+    hipLaunchKernelGGL(kfn, grid, dim3(256), 0, c.stream, c.res,
+                       (const T*)c.u, planes, norm, c.touched, long_, s, jp,
+                       kp);
+  };
+  if (jt == 2) apply(k_thin_apply<T, TALL, 2, 32>);
+  else if (jt == 4) apply(k_thin_apply<T, TALL, 4, 64>);
+  else apply(k_thin_apply<T, TALL, 8, 128>);
 }
 
 template <int NT, typename T>
@@ -793,22 +1196,23 @@ void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
   check_chain(matrix_rows, dim, steps);
   const int64_t batch = table.size(0) / matrix_rows;
   if (!n || !table.numel()) return;
+  const int64_t total = table.size(0);
   c10::DeviceGuard guard(table.device());
   hipStream_t stream = at::hip::getCurrentHIPStream().stream();
   auto touched = at::empty({batch}, table.options().dtype(at::kInt));
-  hipLaunchKernelGGL(k_touched, dim3((batch + 255) / 256), dim3(256), 0,
-                     stream, touched.data_ptr<int>(),
-                     rows.data_ptr<int64_t>(), n, batch, matrix_rows);
   auto u = at::empty_like(table);
-  const int64_t total = table.size(0);
+  int group = 1;
+  while (group < 64 && group * 4 < dim) group *= 2;
+  // long enough chunks to stream, short enough to fill the card
+  const int span = total / 64 >= 1024 ? 64 : 16;
   hipLaunchKernelGGL(k_momentum,
-                     dim3(std::min<int64_t>((total + 3) / 4, 4096)), dim3(256),
-                     0, stream, u.data_ptr<float>(),
+                     dim3(batch * ((matrix_rows + span - 1) / span)),
+                     dim3(256), 0, stream, u.data_ptr<float>(),
                      momentum.data_ptr<float>(), grads.data_ptr<float>(),
                      rows.data_ptr<int64_t>(),
                      order ? order->data_ptr<int64_t>() : nullptr,
-                     touched.data_ptr<int>(), n, total, matrix_rows, dim,
-                     (float)mu, nesterov);
+                     touched.data_ptr<int>(), n, matrix_rows, (int)dim, span,
+                     group, (float)mu, nesterov);
   const double rate = lr * std::sqrt(std::max(1.0, (double)matrix_rows / dim));
   dispatch(Chain{u.data_ptr(), at::kFloat, batch, matrix_rows, dim,
                  touched.data_ptr<int>(), (int)steps, {a, b, c}, eps,
