@@ -24,6 +24,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 #include "ops.h"
@@ -96,23 +97,60 @@ __device__ inline int64_t lower_bound(const int64_t* v, int64_t n,
   return lo;
 }
 
-// M <- mu M + g and U = g + mu M (nesterov) or M for `span` (at most 64) rows
-// of one matrix a block; touched[b] says for the kernels that follow whether
-// the push names a row of matrix b.  g is the sum of the row's gradients in
-// the order of the push: rows are sorted, order[j] is the place of the j-th
-// in `grads`.  Bound by memory: 16 bytes a value.
-__global__ __launch_bounds__(256) void k_momentum(
-    float* __restrict__ u, float* __restrict__ momentum,
-    const float* __restrict__ grads, const int64_t* __restrict__ rows,
-    const int64_t* __restrict__ order, int* __restrict__ touched, int64_t n,
-    int64_t m, int dim, int span, int group, float mu, bool nesterov) {
-  __shared__ int64_t first[64];
+struct Momentum {
+  float* u;
+  float* m;
+  const float* grads;
+  const int64_t* rows;   // sorted
+  const int64_t* order;  // place of the j-th in grads, or null: j
+  int64_t n;
+  float mu;
+  bool nesterov;
+};
+
+// The sum of a row's gradients (at columns c .. c + 3) in the order of the
+// push; `j` is the first of the row's places, < 0 for none.
+__device__ inline float4 row_gradient(const Momentum& q, int64_t j,
+                                      int64_t row, int dim, int c, int held) {
+  if (j < 0) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float4 g = load_quad(q.grads + (q.order ? q.order[j] : j) * dim + c, held);
+  while (++j < q.n && q.rows[j] == row) {
+    const float4 h = load_quad(q.grads + (q.order ? q.order[j] : j) * dim + c,
+                               held);
+    g.x += h.x;
+    g.y += h.y;
+    g.z += h.z;
+    g.w += h.w;
+  }
+  return g;
+}
+
+// M's new value from its old one; u gets U's.
+__device__ inline float4 next_momentum(const Momentum& q, float4 v, float4 g,
+                                       float4* u) {
+  v.x = q.mu * v.x + g.x;
+  v.y = q.mu * v.y + g.y;
+  v.z = q.mu * v.z + g.z;
+  v.w = q.mu * v.w + g.w;
+  *u = q.nesterov ? make_float4(g.x + q.mu * v.x, g.y + q.mu * v.y,
+                                g.z + q.mu * v.z, g.w + q.mu * v.w)
+                  : v;
+  return v;
+}
+
+// first[r] = the first place of row r in the push, -1 for none, for up to 256
+// rows of one matrix a block; touched[b] = whether the push names a row of
+// matrix b.
+__global__ __launch_bounds__(256) void k_places(
+    int64_t* __restrict__ first, int* __restrict__ touched,
+    const int64_t* __restrict__ rows, int64_t n, int64_t m) {
+  __shared__ int64_t mine[256];
   __shared__ int64_t ends[2];
-  const int64_t chunks = (m + span - 1) / span;
+  const int64_t chunks = (m + 255) / 256;
   const int64_t b = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-  const int64_t r0 = b * m + chunk * span;
-  const int64_t count = min((int64_t)span, m - chunk * span);
-  if (threadIdx.x < 64) first[threadIdx.x] = -1;
+  const int64_t r0 = b * m + chunk * 256, count = min(m - chunk * 256,
+                                                      (int64_t)256);
+  mine[threadIdx.x] = -1;
   if (threadIdx.x % WAVE == 0 && threadIdx.x < 2 * WAVE) {
     // a push of every row has row r at place r
     const int64_t x = threadIdx.x == 0 ? r0 : r0 + count;
@@ -121,43 +159,38 @@ __global__ __launch_bounds__(256) void k_momentum(
   }
   __syncthreads();
   const int64_t lo = ends[0], hi = ends[1];
-  bool some = hi > lo;
-  if (!some) {
-    int64_t at = lower_bound(rows, n, b * m);
-    some = at < n && rows[at] < (b + 1) * m;
+  if (chunk == 0 && threadIdx.x == 0) {
+    bool some = hi > lo;
+    if (!some) {
+      const int64_t at = lower_bound(rows, n, b * m);
+      some = at < n && rows[at] < (b + 1) * m;
+    }
+    touched[b] = some;
   }
-  if (chunk == 0 && threadIdx.x == 0) touched[b] = some;
-  if (!some) return;
   for (int64_t j = lo + threadIdx.x; j < hi; j += 256)
-    if (j == lo || rows[j - 1] != rows[j]) first[rows[j] - r0] = j;
+    if (j == lo || rows[j - 1] != rows[j]) mine[rows[j] - r0] = j;
   __syncthreads();
+  if (threadIdx.x < count) first[r0 + threadIdx.x] = mine[threadIdx.x];
+}
+
+// M <- mu M + g and U = g + mu M (nesterov) or M, `group` lanes a row.  Bound
+// by memory: 16 bytes a value.
+__global__ __launch_bounds__(256) void k_momentum(
+    Momentum q, const int64_t* __restrict__ first,
+    const int* __restrict__ touched, int64_t total, int64_t m, int dim,
+    int group) {
   const int lane = threadIdx.x & (group - 1);
-  for (int r = threadIdx.x / group; r < count; r += 256 / group) {
-    const int64_t j0 = first[r], row = r0 + r;
+  for (int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / group;
+       row < total; row += (int64_t)gridDim.x * (256 / group)) {
+    if (!touched[row / m]) continue;
+    const int64_t j = first[row];
     for (int c = lane * 4; c < dim; c += group * 4) {
-      const int held = dim - c;
       const int64_t at = row * dim + c;
-      float4 v = load_quad(momentum + at, held);
-      float4 g = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (j0 >= 0) {
-        g = load_quad(grads + (order ? order[j0] : j0) * dim + c, held);
-        for (int64_t j = j0 + 1; j < hi && rows[j] == row; ++j) {
-          float4 h = load_quad(grads + (order ? order[j] : j) * dim + c, held);
-          g.x += h.x;
-          g.y += h.y;
-          g.z += h.z;
-          g.w += h.w;
-        }
-      }
-      v.x = mu * v.x + g.x;
-      v.y = mu * v.y + g.y;
-      v.z = mu * v.z + g.z;
-      v.w = mu * v.w + g.w;
-      store_quad(momentum + at, v, held);
-      if (nesterov)
-        v = make_float4(g.x + mu * v.x, g.y + mu * v.y, g.z + mu * v.z,
-                        g.w + mu * v.w);
-      store_quad(u + at, v, held);
+      const int held = dim - c;
+      float4 v = load_quad(q.m + at, held), u;
+      v = next_momentum(q, v, row_gradient(q, j, row, dim, c, held), &u);
+      store_quad(q.m + at, v, held);
+      store_quad(q.u + at, u, held);
     }
   }
 }
@@ -224,36 +257,40 @@ __global__ __launch_bounds__(256) void k_gram_narrow(
   f64x4 acc[TILES];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) acc[t] = (f64x4){0, 0, 0, 0};
-#pragma unroll 2
-  for (int64_t k = k0; k < k1; k += 16) {
-    float v[4][NT];
+  constexpr int TURNS = NT > 2 ? 1 : 2;  // 16 places each, loaded together
+  for (int64_t k = k0; k < k1; k += 16 * TURNS) {
+    float v[TURNS][4][NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int col = t * 16 + lane % 16;
-      if (TALL) {
+    for (int h = 0; h < TURNS; ++h)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int64_t kk = k + 4 * c + lane / 16;
-          v[c][t] = col < s && kk < k1 ? to_f32(x[kk * s + col]) : 0.0f;
+      for (int t = 0; t < NT; ++t) {
+        const int col = t * 16 + lane % 16;
+        if (TALL) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int64_t kk = k + h * 16 + 4 * c + lane / 16;
+            v[h][c][t] = col < s && kk < k1 ? to_f32(x[kk * s + col]) : 0.0f;
+          }
+        } else {
+          const int64_t kk = k + h * 16 + lane / 16 * 4;
+          const float4 f = load_quad(x + col * long_ + kk,
+                                     col < s ? k1 - kk : 0);
+          v[h][0][t] = f.x;
+          v[h][1][t] = f.y;
+          v[h][2][t] = f.z;
+          v[h][3][t] = f.w;
         }
-      } else {
-        const int64_t kk = k + lane / 16 * 4;
-        const float4 f = load_quad(x + col * long_ + kk,
-                                   col < s ? k1 - kk : 0);
-        v[0][t] = f.x;
-        v[1][t] = f.y;
-        v[2][t] = f.z;
-        v[3][t] = f.w;
       }
-    }
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int h = 0; h < TURNS; ++h)
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int j = 0; j <= i; ++j)
-          acc[i * (i + 1) / 2 + j] = __builtin_amdgcn_mfma_f64_16x16x4f64(
-              v[c][i], v[c][j], acc[i * (i + 1) / 2 + j], 0, 0, 0);
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int j = 0; j <= i; ++j)
+            acc[i * (i + 1) / 2 + j] = __builtin_amdgcn_mfma_f64_16x16x4f64(
+                v[h][c][i], v[h][c][j], acc[i * (i + 1) / 2 + j], 0, 0, 0);
   }
   for (int w = 0; w < 4; ++w) {
     if (wave == w) {
@@ -276,116 +313,196 @@ __global__ __launch_bounds__(256) void k_gram_narrow(
   }
 }
 
+// KC places of a diagonal square of G, 8 x 8 tiles of which nt x nt exist:
+// wave W takes tile rows W and 7 - W up to the diagonal, nine tiles.
+template <int W>
+__device__ inline void diagonal_places(f64x4 (&acc)[16],
+                                       const float (*rows)[PITCH], int lane,
+                                       int nt) {
+#pragma unroll
+  for (int q = 0; q < KC; q += 4) {
+    const float* at = rows[q + lane / 16] + lane % 16;
+    double v[8 - W];
+#pragma unroll
+    for (int t = 0; t < 8 - W; ++t) v[t] = at[t * 16];
+    if (W < nt) {
+#pragma unroll
+      for (int t = 0; t <= W; ++t)
+        acc[t] = __builtin_amdgcn_mfma_f64_16x16x4f64(v[W], v[t], acc[t], 0,
+                                                      0, 0);
+    }
+    if (7 - W < nt) {
+#pragma unroll
+      for (int t = 0; t <= 7 - W; ++t)
+        acc[W + 1 + t] = __builtin_amdgcn_mfma_f64_16x16x4f64(
+            v[7 - W], v[t], acc[W + 1 + t], 0, 0, 0);
+    }
+  }
+}
+
+// f(tile row, tile column, sum) for each of the nine
+template <int W, typename F>
+__device__ inline void diagonal_tiles(const f64x4 (&acc)[16], F f) {
+#pragma unroll
+  for (int t = 0; t <= W; ++t) f(W, t, acc[t]);
+#pragma unroll
+  for (int t = 0; t <= 7 - W; ++t) f(7 - W, t, acc[W + 1 + t]);
+}
+
+#define BY_WAVE(wave, call)        \
+  switch (wave) {                  \
+    case 0: { constexpr int W = 0; call; } break; \
+    case 1: { constexpr int W = 1; call; } break; \
+    case 2: { constexpr int W = 2; call; } break; \
+    default: { constexpr int W = 3; call; } break; \
+  }
+
 // The same for short sides up to THIN_MAX: a block takes the places of one
-// chunk for a SUPER x SUPER square of G, through LDS.  The matrix
-// instructions bound it: 64 cycles a tile and 4 places.
-template <typename T, bool TALL>
+// chunk for a SUPER x SUPER square of G, through LDS (two buffers, one barrier
+// a turn).  The matrix instructions bound it: 64 cycles a tile and 4 places.
+//
+// With STEP (tall, one square) the values are those of U as the momentum
+// makes it: M and the gradients come in, M and U go out on the way.
+template <typename T, bool TALL, bool STEP>
 __global__ __launch_bounds__(256) void k_gram64(
     double* __restrict__ part, double* __restrict__ traces,
-    const T* __restrict__ u, const int* __restrict__ touched, int64_t long_,
-    int s, int sp, int64_t chunk) {
-  __shared__ float rows_[KC][PITCH], cols_[KC][PITCH];
+    const T* __restrict__ u, Momentum mom, const int64_t* __restrict__ first,
+    const int* __restrict__ touched, int64_t long_, int s, int sp,
+    int64_t chunk) {
+  __shared__ float lds[STEP ? 2 : 4][KC][PITCH];
   __shared__ double sums[4];
   const int64_t b = blockIdx.z;
   if (touched && !touched[b]) return;
   // blockIdx.y counts the pairs of super-tiles (si >= sj)
-  int si = 0, sj = blockIdx.y;
+  int si = 0, sj = STEP ? 0 : blockIdx.y;
   while (sj > si) { sj -= si + 1; ++si; }
-  const bool diagonal = si == sj;
+  const bool diagonal = STEP || si == sj;
+  const int ni = min(8, sp / 16 - si * 8), nj = min(8, sp / 16 - sj * 8);
   const int lane = threadIdx.x % WAVE, wave = this_wave();
   const T* x = u + b * long_ * s;
   const int64_t k0 = blockIdx.x * chunk;
   const int64_t k1 = min(k0 + chunk, long_);
-  const int pair[2] = {wave, 7 - wave};  // this wave's rows of tiles
 
-  f64x4 acc[2][8];
+  f64x4 acc[16];
 #pragma unroll
-  for (int p = 0; p < 2; ++p)
-#pragma unroll
-    for (int t = 0; t < 8; ++t) acc[p][t] = (f64x4){0, 0, 0, 0};
+  for (int t = 0; t < 16; ++t) acc[t] = (f64x4){0, 0, 0, 0};
 
   // four quads a thread: along the columns (TALL) or along the places
   float4 next[2][4];
-  auto fetch = [&](int o, int base, int64_t k) {
+  auto fetch = [&](int64_t k) {
 #pragma unroll
     for (int l = 0; l < 4; ++l) {
       const int e = threadIdx.x + l * 256;
       const int kk = TALL ? e / 32 : e % 8 * 4, c = TALL ? e % 32 * 4 : e / 8;
-      const int64_t held = TALL ? (k + kk < k1 ? s - base - c : 0)
-                                : (base + c < s ? k1 - k - kk : 0);
-      next[o][l] = load_quad(TALL ? x + (k + kk) * s + base + c
-                                  : x + (int64_t)(base + c) * long_ + k + kk,
-                             held);
+      if (STEP) {
+        const int held = k + kk < k1 ? s - c : 0;
+        const int64_t row = b * long_ + k + kk;
+        next[0][l] = load_quad(mom.m + row * s + c, held);
+        next[1][l] = row_gradient(mom, held > 0 ? first[row] : -1, row, s, c,
+                                  held);
+        continue;
+      }
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        if (o && diagonal) continue;
+        const int col = (o ? sj : si) * SUPER + c;
+        const int64_t held = TALL ? (k + kk < k1 ? s - col : 0)
+                                  : (col < s ? k1 - k - kk : 0);
+        next[o][l] = load_quad(TALL ? x + (k + kk) * s + col
+                                    : x + (int64_t)col * long_ + k + kk,
+                               held);
+      }
     }
   };
-  auto put = [&](float (*to)[PITCH], int o) {
+  auto put = [&](int64_t k, int buffer) {
 #pragma unroll
     for (int l = 0; l < 4; ++l) {
       const int e = threadIdx.x + l * 256;
-      const float4 f = next[o][l];
-      if (TALL) {
-        *(float4*)&to[e / 32][e % 32 * 4] = f;
-      } else {
-        const int kk = e % 8 * 4, c = e / 8;
-        to[kk][c] = f.x;
-        to[kk + 1][c] = f.y;
-        to[kk + 2][c] = f.z;
-        to[kk + 3][c] = f.w;
+      const int kk = TALL ? e / 32 : e % 8 * 4, c = TALL ? e % 32 * 4 : e / 8;
+      if (STEP) {
+        const int held = k + kk < k1 ? s - c : 0;
+        const int64_t at = (b * long_ + k + kk) * s + c;
+        float4 v;
+        const float4 m = next_momentum(mom, next[0][l], next[1][l], &v);
+        store_quad(mom.m + at, m, held);
+        store_quad(mom.u + at, v, held);
+        *(float4*)&lds[buffer][kk][c] = v;
+        continue;
+      }
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        if (o && diagonal) continue;
+        float (*to)[PITCH] = lds[buffer + (STEP ? 0 : o * 2)];
+        const float4 f = next[o][l];
+        if (TALL) {
+          *(float4*)&to[kk][c] = f;
+        } else {
+          to[kk][c] = f.x;
+          to[kk + 1][c] = f.y;
+          to[kk + 2][c] = f.z;
+          to[kk + 3][c] = f.w;
+        }
       }
     }
   };
 
-  fetch(0, si * SUPER, k0);
-  if (!diagonal) fetch(1, sj * SUPER, k0);
+  fetch(k0);
+  put(k0, 0);
+  int buffer = 0;
   for (int64_t k = k0; k < k1; k += KC) {
     __syncthreads();
-    put(rows_, 0);
-    if (!diagonal) put(cols_, 1);
-    __syncthreads();
-    if (k + KC < k1) {
-      fetch(0, si * SUPER, k + KC);
-      if (!diagonal) fetch(1, sj * SUPER, k + KC);
-    }
-    const float (*cols)[PITCH] = diagonal ? rows_ : cols_;
-#pragma unroll 2
-    for (int q = 0; q < KC; q += 4) {
-      const int kk = q + lane / 16;
-      double av[2];
+    const bool more = k + KC < k1;
+    if (more) fetch(k + KC);
+    const float (*rows)[PITCH] = lds[buffer];
+    if (diagonal) {
+      BY_WAVE(wave, diagonal_places<W>(acc, rows, lane, ni))
+    } else {
+      const float (*cols)[PITCH] = lds[buffer + (STEP ? 0 : 2)];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) av[p] = rows_[kk][pair[p] * 16 + lane % 16];
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        double bv = cols[kk][t * 16 + lane % 16];
+      for (int q = 0; q < KC; q += 4) {
+        const int kk = q + lane / 16;
+        double av[2], bv[8];
 #pragma unroll
         for (int p = 0; p < 2; ++p)
-          if ((!diagonal || t <= pair[p]) && si * SUPER + pair[p] * 16 < sp &&
-              sj * SUPER + t * 16 < sp)
-            acc[p][t] = __builtin_amdgcn_mfma_f64_16x16x4f64(av[p], bv,
-                                                             acc[p][t], 0, 0,
-                                                             0);
+          av[p] = rows[kk][(wave + p * 4) * 16 + lane % 16];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) bv[t] = cols[kk][t * 16 + lane % 16];
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          if (wave + p * 4 < ni) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+              acc[p * 8 + t] = __builtin_amdgcn_mfma_f64_16x16x4f64(
+                  av[p], bv[t], acc[p * 8 + t], 0, 0, 0);
+          }
       }
     }
+    if (more) put(k + KC, buffer ^ 1);
+    buffer ^= 1;
   }
   double* out = part + (b * gridDim.x + blockIdx.x) * (int64_t)sp * sp;
   double trace = 0;
+  auto keep = [&](int ti, int tj, const f64x4& v) {
+    if (ti >= ni || tj >= nj) return;
 #pragma unroll
-  for (int p = 0; p < 2; ++p)
-#pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      int i0 = si * SUPER + pair[p] * 16, j0 = sj * SUPER + t * 16;
-      if ((diagonal && t > pair[p]) || i0 >= sp || j0 >= sp) continue;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        int i = i0 + lane / 16 + 4 * r, j = j0 + lane % 16;
-        out[(int64_t)i * sp + j] = acc[p][t][r];
-        if (i == j) trace += acc[p][t][r];
-      }
+    for (int r = 0; r < 4; ++r) {
+      const int i = si * SUPER + ti * 16 + lane / 16 + 4 * r;
+      const int j = sj * SUPER + tj * 16 + lane % 16;
+      out[(int64_t)i * sp + j] = v[r];
+      if (i == j) trace += v[r];
     }
+  };
   if (diagonal) {
+    BY_WAVE(wave, diagonal_tiles<W>(acc, keep))
     trace = block_sum(trace, sums);
     if (threadIdx.x == 0)
       traces[(b * gridDim.x + blockIdx.x) * ((sp + SUPER - 1) / SUPER) + si] =
           trace;
+  } else {
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int t = 0; t < 8; ++t) keep(wave + p * 4, t, acc[p * 8 + t]);
   }
 }
 
@@ -405,19 +522,27 @@ __global__ __launch_bounds__(256) void k_gram_sum(
   const double nu = f.x * f.y;
   if (blockIdx.x == 0 && threadIdx.x == 0)
     norm[b] = Norm{(float)f.x, (float)f.y, 0.0f};
+  // 16 values a block, 16 threads a value
+  __shared__ double slices[16][17];
   const int64_t size = (int64_t)sp * sp;
-  int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= size) return;
-  int i = e / sp, j = e % sp;
-  if (i < j) return;
+  const int64_t e = (int64_t)blockIdx.x * 16 + threadIdx.x % 16;
+  const int i = e / sp, j = e % sp;
   const double* p = part + b * chunks * size + e;
   double sum[4] = {0, 0, 0, 0};
-  int k = 0;
-  for (; k + 4 <= chunks; k += 4)
+  if (i >= j) {
+    int k = threadIdx.x / 16;
+    for (; k + 48 < chunks; k += 64)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) sum[q] += p[(k + q) * size];
-  for (; k < chunks; ++k) sum[0] += p[k * size];
-  const double v = ((sum[0] + sum[1]) + (sum[2] + sum[3])) * nu * nu;
+      for (int q = 0; q < 4; ++q) sum[q] += p[(k + q * 16) * size];
+    for (; k < chunks; k += 16) sum[0] += p[k * size];
+  }
+  slices[threadIdx.x / 16][threadIdx.x % 16] =
+      (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  __syncthreads();
+  if (threadIdx.x >= 16 || i < j) return;
+  double v = 0;
+  for (int q = 0; q < 16; ++q) v += slices[q][threadIdx.x];
+  v *= nu * nu;
   g[b * size + e] = v;
   g[b * size + (int64_t)j * sp + i] = v;
 }
@@ -446,7 +571,6 @@ __global__ __launch_bounds__(256) void k_small_mul(
   const double* xr = job.x + base + (int64_t)(ti * 16 + lane % 16) * sp;
   const double* yr = job.y + base + (int64_t)(tj * 16 + lane % 16) * sp;
   f64x4 acc = (f64x4){0, 0, 0, 0};
-#pragma unroll 2
   for (int kk = wave * 16; kk < sp; kk += 64) {
     const f64x4 xv = *(const f64x4*)(xr + kk + lane / 16 * 4);
     const f64x4 yv = *(const f64x4*)(yr + kk + lane / 16 * 4);
@@ -507,67 +631,88 @@ __global__ __launch_bounds__(1024) void k_small_out(
 }
 
 // The chain for short sides up to 64: one block a matrix, G, Q, P and G Q in
-// LDS; a wave takes every fourth tile on or under the diagonal.
-template <int NT>
-__global__ __launch_bounds__(256) void k_chain(
+// LDS; a wave a tile on or under the diagonal.  What bounds it is the length
+// of the chain: 14 products that wait for each other at five steps.
+template <int NT, int WAVES>
+__global__ __launch_bounds__(WAVES * WAVE) void k_chain(
     _Float16* __restrict__ planes, Norm* __restrict__ norm,
     const double* __restrict__ part, const int* __restrict__ touched,
     int chunks, int s, int steps, Coeffs k, double eps, int jp, int kp) {
   constexpr int SP = NT * 16, LP = SP + 2, TILES = NT * (NT + 1) / 2;
-  constexpr int MINE = (TILES + 3) / 4;
-  __shared__ double g[SP * LP], q[SP * LP], p[SP * LP], t[SP * LP], sums[4];
+  // tiles of two products at a time
+  constexpr int MINE = (2 * TILES + WAVES - 1) / WAVES;
+  __shared__ double g[SP * LP], q[SP * LP], p[SP * LP], t[SP * LP];
+  __shared__ double sums[WAVES];
   const int64_t b = blockIdx.x;
   if (touched && !touched[b]) return;
   const int lane = threadIdx.x % WAVE, wave = this_wave();
   const double* from = part + b * chunks * (int64_t)SP * SP;
-  double trace = 0;
-  for (int e = threadIdx.x; e < SP * SP; e += 256) {
-    const int i = e / SP, j = e % SP;
-    if (i < j) continue;
-    double sum[4] = {0, 0, 0, 0};
-    int c = 0;
-    for (; c + 4 <= chunks; c += 4)
+
+  // the sum of the parts: 256 threads take a value of every tile each, and
+  // every (WAVES / 4)-th part
+  const int slice = wave / 4, e = threadIdx.x % 256;
+  double sum[TILES] = {};
+#pragma unroll 4
+  for (int c = slice; c < chunks; c += WAVES / 4) {
+    int ti = 0, tj = 0;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) sum[w] += from[(int64_t)(c + w) * SP * SP + e];
-    for (; c < chunks; ++c) sum[0] += from[(int64_t)c * SP * SP + e];
-    const double v = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    g[i * LP + j] = v;
-    g[j * LP + i] = v;
-    if (i == j) trace += v;
+    for (int o = 0; o < TILES; ++o) {
+      sum[o] += from[((int64_t)c * SP + ti * 16 + e / 16) * SP + tj * 16 +
+                     e % 16];
+      if (++tj > ti) { tj = 0; ++ti; }
+    }
   }
+  for (int w = 0; w < WAVES / 4; ++w) {
+    if (slice == w) {
+      int ti = 0, tj = 0;
+#pragma unroll
+      for (int o = 0; o < TILES; ++o) {
+        const int i = ti * 16 + e / 16, j = tj * 16 + e % 16;
+        if (i >= j) {
+          double v = sum[o];
+          if (w) v += g[i * LP + j];
+          g[i * LP + j] = v;
+          g[j * LP + i] = v;
+        }
+        if (++tj > ti) { tj = 0; ++ti; }
+      }
+    }
+    __syncthreads();
+  }
+  const double trace = threadIdx.x < SP ? g[threadIdx.x * (LP + 1)] : 0.0;
   const double2 f = norm_factors(block_sum(trace, sums), eps);
   const double nu = f.x * f.y;
   if (threadIdx.x == 0) norm[b] = Norm{(float)f.x, (float)f.y, 0.0f};
-  for (int e = threadIdx.x; e < SP * LP; e += 256)
-    if (e % LP < SP) g[e] *= nu * nu;
+  for (int o = threadIdx.x; o < SP * LP; o += WAVES * WAVE)
+    if (o % LP < SP) g[o] *= nu * nu;
   __syncthreads();
 
-  int ti[MINE], tj[MINE];
-#pragma unroll
-  for (int o = 0; o < MINE; ++o) {
-    ti[o] = 0;
-    tj[o] = wave + o * 4;
-    while (tj[o] > ti[o]) { tj[o] -= ti[o] + 1; ++ti[o]; }
-  }
-  // out = x y, or a I + b x + c x y; `out` may be one of the operands
-  auto mul = [&](double* out, const double* x, const double* y, bool poly) {
+  // One or two products: out = x y, or a I + b x + c x y; `out` may be one of
+  // the operands.
+  struct Job { double* out; const double *x, *y; };
+  auto mul = [&](Job j0, Job j1, bool poly) {
     f64x4 acc[MINE];
 #pragma unroll
     for (int o = 0; o < MINE; ++o) {
       acc[o] = (f64x4){0, 0, 0, 0};
-      if (ti[o] >= NT) continue;
-      const double* xr = x + (ti[o] * 16 + lane % 16) * LP + lane / 16;
-      const double* yr = y + (tj[o] * 16 + lane % 16) * LP + lane / 16;
-#pragma unroll 4
+      int tj = wave + o * WAVES, ti = 0;
+      const bool second = tj >= TILES;
+      if (second) tj -= TILES;
+      const Job job = second ? j1 : j0;
+      if (!job.out || tj >= TILES) continue;
+      while (tj > ti) { tj -= ti + 1; ++ti; }
+      const double* xr = job.x + (ti * 16 + lane % 16) * LP + lane / 16;
+      const double* yr = job.y + (tj * 16 + lane % 16) * LP + lane / 16;
+#pragma unroll
       for (int kk = 0; kk < SP; kk += 4)
         acc[o] = __builtin_amdgcn_mfma_f64_16x16x4f64(xr[kk], yr[kk], acc[o],
                                                       0, 0, 0);
       if (poly) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int i = ti[o] * 16 + lane / 16 + 4 * r;
-          const int j = tj[o] * 16 + lane % 16;
-          acc[o][r] = k.b * x[i * LP + j] + k.c * acc[o][r] +
+          const int i = ti * 16 + lane / 16 + 4 * r;
+          const int j = tj * 16 + lane % 16;
+          acc[o][r] = k.b * job.x[i * LP + j] + k.c * acc[o][r] +
                       (i == j && i < s ? k.a : 0.0);
         }
       }
@@ -575,11 +720,16 @@ __global__ __launch_bounds__(256) void k_chain(
     __syncthreads();
 #pragma unroll
     for (int o = 0; o < MINE; ++o) {
-      if (ti[o] >= NT) continue;
+      int tj = wave + o * WAVES, ti = 0;
+      const bool second = tj >= TILES;
+      if (second) tj -= TILES;
+      double* out = second ? j1.out : j0.out;
+      if (!out || tj >= TILES) continue;
+      while (tj > ti) { tj -= ti + 1; ++ti; }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = ti[o] * 16 + lane / 16 + 4 * r;
-        const int j = tj[o] * 16 + lane % 16;
+        const int i = ti * 16 + lane / 16 + 4 * r;
+        const int j = tj * 16 + lane % 16;
         if (i < j) continue;
         out[i * LP + j] = acc[o][r];
         out[j * LP + i] = acc[o][r];
@@ -587,14 +737,15 @@ __global__ __launch_bounds__(256) void k_chain(
     }
     __syncthreads();
   };
+  const Job none{nullptr, nullptr, nullptr};
   for (int step = 0; step < steps; ++step) {
     double* qi = step ? q : p;  // the first Q is P
-    mul(qi, g, g, true);
-    if (step) mul(p, p, q, false);
-    if (step + 1 < steps) {
-      mul(t, g, qi, false);
-      mul(g, qi, t, false);
-    }
+    mul({qi, g, g}, none, true);
+    const Job grow{t, g, qi}, more{p, p, q};
+    const bool last = step + 1 == steps;
+    if (step) mul(more, last ? none : grow, false);
+    else if (!last) mul(grow, none, false);
+    if (!last) mul({g, qi, t}, none, false);
   }
   put_planes(planes + b * (int64_t)jp * kp, gridDim.x * (int64_t)jp * kp, jp,
              kp, s, [&](int i, int j) { return p[i * LP + j]; }, norm + b,
@@ -953,7 +1104,17 @@ struct Chain {
   Result res;
   at::TensorOptions options;
   hipStream_t stream;
+  // Muon: U comes from these; with `fused` the pass that sums G makes it,
+  // without it is there
+  bool fused = false;
+  Momentum momentum{};
+  const int64_t* first = nullptr;
 };
+
+bool is_thin(int64_t m, int64_t n) {
+  const int64_t s = std::min(m, n), long_ = std::max(m, n);
+  return s <= NARROW || (s <= THIN_MAX && long_ >= 32 * s);
+}
 
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
@@ -984,27 +1145,36 @@ void run_thin(const Chain& c) {
   Norm* norm = (Norm*)nm.data_ptr();
   double* parts = part.data_ptr<double>();
   if (narrow) {
-    auto go = [&](auto* gram, auto* chain) {
+    auto go = [&](auto* gram, auto* chain, int threads) {
       hipLaunchKernelGGL(gram, dim3(chunks, c.batch), dim3(256), 0, c.stream,
                          parts, (const T*)c.u, c.touched, long_, s, chunk);
-      hipLaunchKernelGGL(chain, dim3(c.batch), dim3(256), 0, c.stream, planes,
+      hipLaunchKernelGGL(chain, dim3(c.batch), dim3(threads), 0, c.stream, planes,
                          norm, parts, c.touched, (int)chunks, s, c.steps, c.k,
                          c.eps, jp, kp);
     };
-    if (nt == 1) go(k_gram_narrow<T, TALL, 1>, k_chain<1>);
-    else if (nt == 2) go(k_gram_narrow<T, TALL, 2>, k_chain<2>);
-    else go(k_gram_narrow<T, TALL, 4>, k_chain<4>);
+    if (nt == 1) go(k_gram_narrow<T, TALL, 1>, k_chain<1, 4>, 256);
+    else if (nt == 2) go(k_gram_narrow<T, TALL, 2>, k_chain<2, 16>, 1024);
+    else go(k_gram_narrow<T, TALL, 4>, k_chain<4, 16>, 1024);
   } else {
     auto tr = at::empty({c.batch * chunks * super}, f64);
     auto work = at::empty({6, c.batch * size}, f64);
     double* w[6];
     for (int i = 0; i < 6; ++i)
       w[i] = work.data_ptr<double>() + i * c.batch * size;
-    hipLaunchKernelGGL((k_gram64<T, TALL>), dim3(chunks, pairs, c.batch),
-                       dim3(256), 0, c.stream, parts, tr.data_ptr<double>(),
-                       (const T*)c.u, c.touched, long_, s, sp, chunk);
+    auto gram = [&](auto* kfn, const Momentum& q, const int64_t* first) {
+      hipLaunchKernelGGL(kfn, dim3(chunks, pairs, c.batch), dim3(256), 0,
+                         c.stream, parts, tr.data_ptr<double>(),
+                         (const T*)c.u, q, first, c.touched, long_, s, sp,
+                         chunk);
+    };
+    if constexpr (TALL && std::is_same_v<T, float>) {
+      if (c.fused) gram(k_gram64<T, TALL, true>, c.momentum, c.first);
+      else gram(k_gram64<T, TALL, false>, {}, nullptr);
+    } else {
+      gram(k_gram64<T, TALL, false>, {}, nullptr);
+    }
     double *g = w[0], *q = w[1], *p = w[2], *t = w[3], *g2 = w[4], *p2 = w[5];
-    hipLaunchKernelGGL(k_gram_sum, dim3((size + 255) / 256, c.batch),
+    hipLaunchKernelGGL(k_gram_sum, dim3(size / 16, c.batch),
                        dim3(256), 0, c.stream, g, norm, parts,
                        tr.data_ptr<double>(), c.touched, (int)chunks, sp,
                        c.eps);
@@ -1118,8 +1288,7 @@ void run_wide(const Chain& c) {
 
 template <typename T>
 void run(const Chain& c) {
-  const int64_t s = std::min(c.m, c.n), long_ = std::max(c.m, c.n);
-  if (s <= 64 || (s <= THIN_MAX && long_ >= 32 * s)) {
+  if (is_thin(c.m, c.n)) {
     if (c.m >= c.n) run_thin<T, true>(c); else run_thin<T, false>(c);
   } else {
     run_wide<T>(c);
@@ -1201,22 +1370,37 @@ void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
   hipStream_t stream = at::hip::getCurrentHIPStream().stream();
   auto touched = at::empty({batch}, table.options().dtype(at::kInt));
   auto u = at::empty_like(table);
-  int group = 1;
-  while (group < 64 && group * 4 < dim) group *= 2;
-  // long enough chunks to stream, short enough to fill the card
-  const int span = total / 64 >= 1024 ? 64 : 16;
-  hipLaunchKernelGGL(k_momentum,
-                     dim3(batch * ((matrix_rows + span - 1) / span)),
-                     dim3(256), 0, stream, u.data_ptr<float>(),
-                     momentum.data_ptr<float>(), grads.data_ptr<float>(),
-                     rows.data_ptr<int64_t>(),
-                     order ? order->data_ptr<int64_t>() : nullptr,
-                     touched.data_ptr<int>(), n, matrix_rows, (int)dim, span,
-                     group, (float)mu, nesterov);
+  auto first = at::empty({total}, rows.options());
+  hipLaunchKernelGGL(k_places,
+                     dim3(batch * ((matrix_rows + 255) / 256)), dim3(256), 0,
+                     stream, first.data_ptr<int64_t>(),
+                     touched.data_ptr<int>(), rows.data_ptr<int64_t>(), n,
+                     matrix_rows);
+  const Momentum q{u.data_ptr<float>(),       momentum.data_ptr<float>(),
+                   grads.data_ptr<float>(),   rows.data_ptr<int64_t>(),
+                   order ? order->data_ptr<int64_t>() : nullptr,
+                   n,                         (float)mu,
+                   nesterov};
+  // one pass makes U and sums G where a block holds a row and a square of G
+  const bool fused = is_thin(matrix_rows, dim) && dim > NARROW &&
+                     dim <= SUPER && matrix_rows >= dim && batch <= 32768;
+  if (!fused) {
+    int group = 1;
+    while (group < 64 && group * 4 < dim) group *= 2;
+    const int64_t blocks = (total * group + 255) / 256;
+    hipLaunchKernelGGL(k_momentum, dim3(std::min<int64_t>(blocks, 8192)),
+                       dim3(256), 0, stream, q, first.data_ptr<int64_t>(),
+                       touched.data_ptr<int>(), total, matrix_rows, (int)dim,
+                       group);
+  }
   const double rate = lr * std::sqrt(std::max(1.0, (double)matrix_rows / dim));
-  dispatch(Chain{u.data_ptr(), at::kFloat, batch, matrix_rows, dim,
-                 touched.data_ptr<int>(), (int)steps, {a, b, c}, eps,
-                 {table.data_ptr(), (float)(1.0 - lr * weight_decay),
-                  (float)rate, true},
-                 table.options(), stream});
+  Chain chain{u.data_ptr(), at::kFloat, batch, matrix_rows, dim,
+              touched.data_ptr<int>(), (int)steps, {a, b, c}, eps,
+              {table.data_ptr(), (float)(1.0 - lr * weight_decay),
+               (float)rate, true},
+              table.options(), stream};
+  chain.fused = fused;
+  chain.momentum = q;
+  chain.first = first.data_ptr<int64_t>();
+  dispatch(chain);
 }
