@@ -108,20 +108,25 @@ struct Momentum {
   bool nesterov;
 };
 
+// Where a row's gradient is: its place in grads (>= 0), nowhere (-1), or, for
+// several, -2 - j with j the first of them in the sorted push.  Said before
+// the values are wanted, so that no load of those waits for a comparison.
+__device__ inline int64_t several(int64_t j) { return -2 - j; }
+
 // The sum of a row's gradients (at columns c .. c + 3) in the order of the
-// push; `j` is the first of the row's places, < 0 for none.
-__device__ inline float4 row_gradient(const Momentum& q, int64_t j,
+// push.
+__device__ inline float4 row_gradient(const Momentum& q, int64_t place,
                                       int64_t row, int dim, int c, int held) {
-  if (j < 0) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float4 g = load_quad(q.grads + (q.order ? q.order[j] : j) * dim + c, held);
-  while (++j < q.n && q.rows[j] == row) {
-    const float4 h = load_quad(q.grads + (q.order ? q.order[j] : j) * dim + c,
-                               held);
-    g.x += h.x;
-    g.y += h.y;
-    g.z += h.z;
-    g.w += h.w;
-  }
+  float4 g = load_quad(q.grads + place * dim + c, place >= 0 ? held : 0);
+  if (place < -1)
+    for (int64_t j = several(place); j < q.n && q.rows[j] == row; ++j) {
+      const float4 h = load_quad(
+          q.grads + (q.order ? q.order[j] : j) * dim + c, held);
+      g.x += h.x;
+      g.y += h.y;
+      g.z += h.z;
+      g.w += h.w;
+    }
   return g;
 }
 
@@ -138,12 +143,12 @@ __device__ inline float4 next_momentum(const Momentum& q, float4 v, float4 g,
   return v;
 }
 
-// first[r] = the first place of row r in the push, -1 for none, for up to 256
-// rows of one matrix a block; touched[b] = whether the push names a row of
-// matrix b.
+// place[r] (see several()) for up to 256 rows of one matrix a block;
+// touched[b] = whether the push names a row of matrix b.
 __global__ __launch_bounds__(256) void k_places(
-    int64_t* __restrict__ first, int* __restrict__ touched,
-    const int64_t* __restrict__ rows, int64_t n, int64_t m) {
+    int64_t* __restrict__ place, int* __restrict__ touched,
+    const int64_t* __restrict__ rows, const int64_t* __restrict__ order,
+    int64_t n, int64_t m) {
   __shared__ int64_t mine[256];
   __shared__ int64_t ends[2];
   const int64_t chunks = (m + 255) / 256;
@@ -168,22 +173,25 @@ __global__ __launch_bounds__(256) void k_places(
     touched[b] = some;
   }
   for (int64_t j = lo + threadIdx.x; j < hi; j += 256)
-    if (j == lo || rows[j - 1] != rows[j]) mine[rows[j] - r0] = j;
+    if (j == lo || rows[j - 1] != rows[j])
+      mine[rows[j] - r0] = j + 1 < hi && rows[j + 1] == rows[j]
+                               ? several(j)
+                               : (order ? order[j] : j);
   __syncthreads();
-  if (threadIdx.x < count) first[r0 + threadIdx.x] = mine[threadIdx.x];
+  if (threadIdx.x < count) place[r0 + threadIdx.x] = mine[threadIdx.x];
 }
 
 // M <- mu M + g and U = g + mu M (nesterov) or M, `group` lanes a row.  Bound
 // by memory: 16 bytes a value.
 __global__ __launch_bounds__(256) void k_momentum(
-    Momentum q, const int64_t* __restrict__ first,
+    Momentum q, const int64_t* __restrict__ place,
     const int* __restrict__ touched, int64_t total, int64_t m, int dim,
     int group) {
   const int lane = threadIdx.x & (group - 1);
   for (int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / group;
        row < total; row += (int64_t)gridDim.x * (256 / group)) {
     if (!touched[row / m]) continue;
-    const int64_t j = first[row];
+    const int64_t j = place[row];
     for (int c = lane * 4; c < dim; c += group * 4) {
       const int64_t at = row * dim + c;
       const int held = dim - c;
@@ -315,8 +323,8 @@ __global__ __launch_bounds__(256) void k_gram_narrow(
 
 // KC places of a diagonal square of G, 8 x 8 tiles of which nt x nt exist:
 // wave W takes tile rows W and 7 - W up to the diagonal, nine tiles.
-template <int W>
-__device__ inline void diagonal_places(f64x4 (&acc)[16],
+template <int W, int N>
+__device__ inline void diagonal_places(f64x4 (&acc)[N],
                                        const float (*rows)[PITCH], int lane,
                                        int nt) {
 #pragma unroll
@@ -341,8 +349,8 @@ __device__ inline void diagonal_places(f64x4 (&acc)[16],
 }
 
 // f(tile row, tile column, sum) for each of the nine
-template <int W, typename F>
-__device__ inline void diagonal_tiles(const f64x4 (&acc)[16], F f) {
+template <int W, int N, typename F>
+__device__ inline void diagonal_tiles(const f64x4 (&acc)[N], F f) {
 #pragma unroll
   for (int t = 0; t <= W; ++t) f(W, t, acc[t]);
 #pragma unroll
@@ -364,9 +372,9 @@ __device__ inline void diagonal_tiles(const f64x4 (&acc)[16], F f) {
 // With STEP (tall, one square) the values are those of U as the momentum
 // makes it: M and the gradients come in, M and U go out on the way.
 template <typename T, bool TALL, bool STEP>
-__global__ __launch_bounds__(256) void k_gram64(
+__global__ __launch_bounds__(256, STEP ? 2 : 1) void k_gram64(
     double* __restrict__ part, double* __restrict__ traces,
-    const T* __restrict__ u, Momentum mom, const int64_t* __restrict__ first,
+    const T* __restrict__ u, Momentum mom, const int64_t* __restrict__ place,
     const int* __restrict__ touched, int64_t long_, int s, int sp,
     int64_t chunk) {
   __shared__ float lds[STEP ? 2 : 4][KC][PITCH];
@@ -383,9 +391,20 @@ __global__ __launch_bounds__(256) void k_gram64(
   const int64_t k0 = blockIdx.x * chunk;
   const int64_t k1 = min(k0 + chunk, long_);
 
-  f64x4 acc[16];
+  constexpr int TILES = STEP ? 9 : 16;  // a wave's, at most
+  f64x4 acc[TILES];
 #pragma unroll
-  for (int t = 0; t < 16; ++t) acc[t] = (f64x4){0, 0, 0, 0};
+  for (int t = 0; t < TILES; ++t) acc[t] = (f64x4){0, 0, 0, 0};
+
+  // STEP: the places are known a turn ahead of the values
+  int64_t at_[4];
+  auto look = [&](int64_t k) {
+#pragma unroll
+    for (int l = 0; l < 4; ++l) {
+      const int64_t kk = k + (threadIdx.x + l * 256) / 32;
+      at_[l] = STEP && kk < k1 ? place[b * long_ + kk] : -1;
+    }
+  };
 
   // four quads a thread: along the columns (TALL) or along the places
   float4 next[2][4];
@@ -398,8 +417,7 @@ __global__ __launch_bounds__(256) void k_gram64(
         const int held = k + kk < k1 ? s - c : 0;
         const int64_t row = b * long_ + k + kk;
         next[0][l] = load_quad(mom.m + row * s + c, held);
-        next[1][l] = row_gradient(mom, held > 0 ? first[row] : -1, row, s, c,
-                                  held);
+        next[1][l] = row_gradient(mom, at_[l], row, s, c, held);
         continue;
       }
 #pragma unroll
@@ -446,18 +464,23 @@ __global__ __launch_bounds__(256) void k_gram64(
     }
   };
 
+  look(k0);
   fetch(k0);
+  look(k0 + KC);
   put(k0, 0);
   int buffer = 0;
   for (int64_t k = k0; k < k1; k += KC) {
     __syncthreads();
     const bool more = k + KC < k1;
-    if (more) fetch(k + KC);
+    if (more) {
+      fetch(k + KC);
+      look(k + 2 * KC);
+    }
     const float (*rows)[PITCH] = lds[buffer];
     if (diagonal) {
       BY_WAVE(wave, diagonal_places<W>(acc, rows, lane, ni))
-    } else {
-      const float (*cols)[PITCH] = lds[buffer + (STEP ? 0 : 2)];
+    } else if constexpr (!STEP) {
+      const float (*cols)[PITCH] = lds[buffer + 2];
 #pragma unroll
       for (int q = 0; q < KC; q += 4) {
         const int kk = q + lane / 16;
@@ -498,7 +521,7 @@ __global__ __launch_bounds__(256) void k_gram64(
     if (threadIdx.x == 0)
       traces[(b * gridDim.x + blockIdx.x) * ((sp + SUPER - 1) / SUPER) + si] =
           trace;
-  } else {
+  } else if constexpr (!STEP) {
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
@@ -1108,7 +1131,7 @@ struct Chain {
   // without it is there
   bool fused = false;
   Momentum momentum{};
-  const int64_t* first = nullptr;
+  const int64_t* place = nullptr;
 };
 
 bool is_thin(int64_t m, int64_t n) {
@@ -1161,14 +1184,14 @@ void run_thin(const Chain& c) {
     double* w[6];
     for (int i = 0; i < 6; ++i)
       w[i] = work.data_ptr<double>() + i * c.batch * size;
-    auto gram = [&](auto* kfn, const Momentum& q, const int64_t* first) {
+    auto gram = [&](auto* kfn, const Momentum& q, const int64_t* place) {
       hipLaunchKernelGGL(kfn, dim3(chunks, pairs, c.batch), dim3(256), 0,
                          c.stream, parts, tr.data_ptr<double>(),
-                         (const T*)c.u, q, first, c.touched, long_, s, sp,
+                         (const T*)c.u, q, place, c.touched, long_, s, sp,
                          chunk);
     };
     if constexpr (TALL && std::is_same_v<T, float>) {
-      if (c.fused) gram(k_gram64<T, TALL, true>, c.momentum, c.first);
+      if (c.fused) gram(k_gram64<T, TALL, true>, c.momentum, c.place);
       else gram(k_gram64<T, TALL, false>, {}, nullptr);
     } else {
       gram(k_gram64<T, TALL, false>, {}, nullptr);
@@ -1370,11 +1393,12 @@ void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
   hipStream_t stream = at::hip::getCurrentHIPStream().stream();
   auto touched = at::empty({batch}, table.options().dtype(at::kInt));
   auto u = at::empty_like(table);
-  auto first = at::empty({total}, rows.options());
+  auto place = at::empty({total}, rows.options());
   hipLaunchKernelGGL(k_places,
                      dim3(batch * ((matrix_rows + 255) / 256)), dim3(256), 0,
-                     stream, first.data_ptr<int64_t>(),
-                     touched.data_ptr<int>(), rows.data_ptr<int64_t>(), n,
+                     stream, place.data_ptr<int64_t>(),
+                     touched.data_ptr<int>(), rows.data_ptr<int64_t>(),
+                     order ? order->data_ptr<int64_t>() : nullptr, n,
                      matrix_rows);
   const Momentum q{u.data_ptr<float>(),       momentum.data_ptr<float>(),
                    grads.data_ptr<float>(),   rows.data_ptr<int64_t>(),
@@ -1389,7 +1413,7 @@ void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
     while (group < 64 && group * 4 < dim) group *= 2;
     const int64_t blocks = (total * group + 255) / 256;
     hipLaunchKernelGGL(k_momentum, dim3(std::min<int64_t>(blocks, 8192)),
-                       dim3(256), 0, stream, q, first.data_ptr<int64_t>(),
+                       dim3(256), 0, stream, q, place.data_ptr<int64_t>(),
                        touched.data_ptr<int>(), total, matrix_rows, (int)dim,
                        group);
   }
@@ -1401,6 +1425,6 @@ void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
               table.options(), stream};
   chain.fused = fused;
   chain.momentum = q;
-  chain.first = first.data_ptr<int64_t>();
+  chain.place = place.data_ptr<int64_t>();
   dispatch(chain);
 }
