@@ -915,33 +915,20 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_sumsq(
     double* __restrict__ part, const T* __restrict__ u,
     const int* __restrict__ touched, int64_t size) {
-  __shared__ double lds[256];
+  __shared__ double lds[4];
   const int64_t b = blockIdx.y;
   if (touched && !touched[b]) return;
+  const T* x = u + b * size;
   double t = 0;
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < size;
-       e += (int64_t)gridDim.x * 256) {
-    double v = to_f32(u[b * size + e]);
-    t += v * v;
+#pragma unroll 4
+  for (int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; e < size;
+       e += (int64_t)gridDim.x * 1024) {
+    const float4 f = load_quad(x + e, size - e);
+    t += ((double)f.x * f.x + (double)f.y * f.y) +
+         ((double)f.z * f.z + (double)f.w * f.w);
   }
-  lds[threadIdx.x] = t;
-  __syncthreads();
-  for (int o = 128; o; o >>= 1) {
-    if (threadIdx.x < o) lds[threadIdx.x] += lds[threadIdx.x + o];
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) part[b * gridDim.x + blockIdx.x] = lds[0];
-}
-
-__global__ __launch_bounds__(256) void k_norm(
-    float2* __restrict__ scale, const double* __restrict__ part, int parts,
-    int64_t batch, double eps) {
-  int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (b >= batch) return;
-  double t = 0;
-  for (int k = 0; k < parts; ++k) t += part[b * parts + k];
-  const double2 f = norm_factors(t, eps);
-  scale[b] = make_float2((float)f.x, (float)f.y);
+  t = block_sum(t, lds);
+  if (threadIdx.x == 0) part[b * gridDim.x + blockIdx.x] = t;
 }
 
 // The planes of X as it lies in memory (m x n) and transposed, 64 x 64 values
@@ -949,12 +936,16 @@ __global__ __launch_bounds__(256) void k_norm(
 template <typename T>
 __global__ __launch_bounds__(256) void k_planes(
     Planes nat, Planes trn, const T* __restrict__ u,
-    const float2* __restrict__ scale, const int* __restrict__ touched,
-    int64_t m, int64_t n) {
+    const double* __restrict__ part, int parts,
+    const int* __restrict__ touched, int64_t m, int64_t n, double eps) {
   __shared__ float lds[64][65];
+  __shared__ double sums[4];
   const int64_t b = blockIdx.z;
   if (touched && !touched[b]) return;
-  const float2 sc = scale[b];
+  double t = 0;
+  for (int k = threadIdx.x; k < parts; k += 256) t += part[b * parts + k];
+  const double2 f = norm_factors(block_sum(t, sums), eps);
+  const float2 sc = make_float2((float)f.x, (float)f.y);
   const int64_t wide = nat.pitch / 64;
   const int64_t r0 = blockIdx.x / wide * 64, c0 = blockIdx.x % wide * 64;
   for (int e = threadIdx.x; e < 64 * 64; e += 256) {
@@ -985,45 +976,199 @@ struct Product {
   int64_t rows, cols;  // FINAL: D's own size
   bool tall;           // FINAL: D transposed is what lies in memory
   Result res;
+  // the work: tiles of one matrix (ns rows of them, nl columns), matrices;
+  // of all tiles the first `whole` are a block's each, the others have their
+  // sum shared out to `splits` blocks, which leave it in `parts`
+  int ns, nl, tiles, splits;
+  int64_t all, whole;
+  float* parts;
 };
 
-// One block an NT x NT tile of D, four waves a quarter each, 32 places of K
-// at a time through LDS.  LDS rows are four 16-byte pieces; piece c of row r
-// lies at c ^ (r / 2 % 4), so that eight lanes that read one piece of eight
-// rows hit different banks.
-template <int NT, Ending E, typename T>
-__global__ __launch_bounds__(256) void k_product(
-    Product pr, const int* __restrict__ touched) {
-  constexpr int W = NT / 32;               // 16-tiles a wave on each side
-  constexpr int LOADS = NT * 4 / 256;      // 16-byte pieces a thread and plane
-  __shared__ half8 lds[2][2][NT * 4];      // operand, plane
-  const int64_t b = blockIdx.z;
-  if (touched && !touched[b]) return;
-  int bi = blockIdx.y, bj = blockIdx.x;
-  if (E == GRAM || E == POLY) {
-    bi = 0;
-    while (bj > bi) { bj -= bi + 1; ++bi; }
+constexpr int XCDS = 8;   // block b runs on XCD b % 8, each with its own L2
+constexpr int STRIP = 8;  // tiles are taken in strips of eight columns
+
+// Tile t of the ns x nl tiles, or (HALF) of those on and under the diagonal
+// of ns x ns: strips of STRIP columns, a strip's rows one after the other, so
+// that neighbours in t share their operands' rows.
+template <bool HALF>
+__device__ inline void tile_of(int t, int ns, int nl, int* bi, int* bj) {
+  if (!HALF) {
+    const int strip = t / (ns * STRIP), rest = t - strip * ns * STRIP;
+    const int wide = min(STRIP, nl - strip * STRIP);
+    *bi = rest / wide;
+    *bj = strip * STRIP + rest % wide;
+    return;
   }
+  int c0 = 0;
+  for (;;) {
+    const int wide = min(STRIP, ns - c0), head = wide * (wide + 1) / 2;
+    const int size = head + max(0, ns - c0 - STRIP) * STRIP;
+    if (t < size) {
+      if (t >= head) {
+        *bi = c0 + STRIP + (t - head) / STRIP;
+        *bj = c0 + (t - head) % STRIP;
+      } else {
+        int i = 0;
+        while (t > i) { t -= i + 1; ++i; }
+        *bi = c0 + i;
+        *bj = c0 + t;
+      }
+      return;
+    }
+    t -= size;
+    c0 += STRIP;
+  }
+}
+
+// What one block leaves of its tile: a lane holds D[i .. i + 3][j] of each
+// 16 x 16 tile of its wave's quarter.  `lds` is free to be written.
+template <int NT, Ending E, typename T>
+__device__ inline void end_product(const Product& pr, int64_t b, int bi,
+                                   int bj, f32x4 (&acc)[NT / 32][NT / 32],
+                                   _Float16* lds) {
+  constexpr int W = NT / 32;
   const int lane = threadIdx.x % WAVE, wave = this_wave();
   const int wi = wave / 2 * (NT / 2), wj = wave % 2 * (NT / 2);
+  if (E == FINAL) {
+#pragma unroll
+    for (int ti = 0; ti < W; ++ti)
+#pragma unroll
+      for (int tj = 0; tj < W; ++tj) {
+        const int64_t i = (int64_t)bi * NT + wi + ti * 16 + lane / 16 * 4;
+        const int64_t j = (int64_t)bj * NT + wj + tj * 16 + lane % 16;
+        if (j >= pr.cols) continue;
+        const f32x4 v = acc[ti][tj] * (1.0f / (UP * UP));
+        const int64_t base = b * pr.rows * pr.cols;
+        if (pr.tall) {
+          finish_quad<T>(pr.res, base + j * pr.rows + i,
+                         make_float4(v[0], v[1], v[2], v[3]), pr.rows - i);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (i + r < pr.rows)
+              finish<T>(pr.res, base + (i + r) * pr.cols + j, v[r]);
+        }
+      }
+    return;
+  }
+  // D as it is goes out through LDS, in 16-byte pieces; D transposed, four
+  // values a lane, from the registers.
+  constexpr int ROW = NT + 8;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    __syncthreads();
+#pragma unroll
+    for (int ti = 0; ti < W; ++ti)
+#pragma unroll
+      for (int tj = 0; tj < W; ++tj) {
+        const int li = wi + ti * 16 + lane / 16 * 4;
+        const int lj = wj + tj * 16 + lane % 16;
+        const int64_t i = (int64_t)bi * NT + li, j = (int64_t)bj * NT + lj;
+        if (h == 0) {
+          f32x4 v = acc[ti][tj] * (1.0f / UP);
+          if (E == POLY) {
+            // a is symmetric: its row j has the four values side by side
+            const _Float16* g = pr.a.p + b * pr.a.batch + j * pr.a.pitch + i;
+            const half4 gh = *(const half4*)g;
+            const half4 gl = *(const half4*)(g + pr.a.plane);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              v[r] = pr.cc * v[r] + pr.cb * ((float)gh[r] + (float)gl[r]);
+              if (i + r == j && j < pr.s) v[r] += pr.ca * UP;
+            }
+          }
+          acc[ti][tj] = v;
+        }
+        half4 w;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          _Float16 hi, lo;
+          split(acc[ti][tj][r], hi, lo);
+          w[r] = h ? lo : hi;
+          lds[(li + r) * ROW + lj] = w[r];
+        }
+        if (E == UPDATE || bi != bj) {
+          const Planes& t = E == UPDATE ? pr.dt : pr.d;
+          *(half4*)(t.p + h * t.plane + b * t.batch + j * t.pitch + i) = w;
+        }
+      }
+    __syncthreads();
+    for (int e = threadIdx.x; e < NT * NT / 8; e += 256) {
+      const int r = e / (NT / 8), c = e % (NT / 8) * 8;
+      *(half8*)(pr.d.p + h * pr.d.plane + b * pr.d.batch +
+                ((int64_t)bi * NT + r) * pr.d.pitch + (int64_t)bj * NT + c) =
+          *(const half8*)(lds + r * ROW + c);
+    }
+  }
+}
+
+// A block an NT x NT tile of D (or its share of the sum), four waves a quarter
+// each, 32 places of K at a time: while the matrix instructions work on one of
+// the LDS buffers, the places that follow go from memory to the others without
+// a stop in registers.  A row of a buffer is four 16-byte pieces; piece c of
+// row r lies at c ^ (r / 2 % 4), so that eight lanes that read one piece of
+// eight rows hit different banks.  Three products of 16 cycles for each pair of
+// 16 x 16 x 32 operands.
+template <int NT, int BUFFERS, Ending E, typename T>
+__global__ __launch_bounds__(256, 2) void k_product(
+    Product pr, const int* __restrict__ touched) {
+  constexpr bool HALF = E == GRAM || E == POLY;
+  constexpr int W = NT / 32;           // 16-tiles a wave on each side
+  constexpr int LOADS = NT / 64;       // pieces a thread, operand and plane
+  __shared__ half8 lds[BUFFERS][2][2][NT * 4];  // buffer, operand, plane
+  static_assert(NT * (NT + 8) * sizeof(_Float16) <= sizeof(lds), "");
+
+  // each XCD takes one run of the whole tiles, and one of the shares
+  int64_t id = blockIdx.x, count = pr.whole, tile;
+  int part = 0, splits = 1;
+  const bool shared = id >= (pr.whole + XCDS - 1) / XCDS * XCDS;
+  if (shared) {
+    id -= (pr.whole + XCDS - 1) / XCDS * XCDS;
+    splits = pr.splits;
+    count = (pr.all - pr.whole) * splits;
+  }
+  const int64_t each = (count + XCDS - 1) / XCDS;
+  id = id % XCDS * each + id / XCDS;
+  if (id >= count) return;
+  tile = id / splits;
+  part = id % splits;
+  float* parts = pr.parts + id * (NT * NT);
+  if (shared) tile += pr.whole;
+  const int64_t b = tile / pr.tiles;
+  if (touched && !touched[b]) return;
+  int bi, bj;
+  tile_of<HALF>(tile % pr.tiles, pr.ns, pr.nl, &bi, &bj);
+
+  const int lane = threadIdx.x % WAVE, wave = this_wave();
+  const int wi = wave / 2 * (NT / 2), wj = wave % 2 * (NT / 2);
+  const int first = (int64_t)(pr.k / 32) * part / splits;
+  const int steps = (int)((int64_t)(pr.k / 32) * (part + 1) / splits) - first;
 
   const _Float16* src[2] = {
-      pr.a.p + b * pr.a.batch + (int64_t)bi * NT * pr.a.pitch,
-      pr.b.p + b * pr.b.batch + (int64_t)bj * NT * pr.b.pitch};
-  const int64_t pitch[2] = {pr.a.pitch, pr.b.pitch};
+      pr.a.p + b * pr.a.batch + (int64_t)bi * NT * pr.a.pitch + first * 32,
+      pr.b.p + b * pr.b.batch + (int64_t)bj * NT * pr.b.pitch + first * 32};
   const int64_t plane[2] = {pr.a.plane, pr.b.plane};
-
-  half8 next[2][2][LOADS];
-  auto fetch = [&](int k) {
+  int64_t from[2][LOADS];
+#pragma unroll
+  for (int l = 0; l < LOADS; ++l) {
+    const int e = (l * 4 + wave) * WAVE + lane, r = e / 4;
+    const int c = (e % 4 ^ (r / 2 % 4)) * 8;
+    from[0][l] = r * pr.a.pitch + c;
+    from[1][l] = r * pr.b.pitch + c;
+  }
+  auto fetch = [&](int step, int buffer) {
 #pragma unroll
     for (int o = 0; o < 2; ++o)
 #pragma unroll
-      for (int l = 0; l < LOADS; ++l) {
-        int e = threadIdx.x + l * 256, r = e / 4, c = e % 4;
-        const _Float16* at = src[o] + r * pitch[o] + k + c * 8;
-        next[o][0][l] = *(const half8*)at;
-        next[o][1][l] = *(const half8*)(at + plane[o]);
-      }
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int l = 0; l < LOADS; ++l)
+          __builtin_amdgcn_global_load_lds(
+              (const __attribute__((address_space(1))) void*)(
+                  src[o] + h * plane[o] + from[o][l] + step * 32),
+              (__attribute__((address_space(3))) void*)&lds[buffer][o][h]
+                  [(l * 4 + wave) * WAVE],
+              16, 0, 0);
   };
 
   f32x4 acc[W][W];
@@ -1032,27 +1177,30 @@ __global__ __launch_bounds__(256) void k_product(
 #pragma unroll
     for (int j = 0; j < W; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
 
-  fetch(0);
-  for (int k = 0; k < pr.k; k += 32) {
-    __syncthreads();
 #pragma unroll
-    for (int o = 0; o < 2; ++o)
-#pragma unroll
-      for (int l = 0; l < LOADS; ++l) {
-        int e = threadIdx.x + l * 256, r = e / 4, c = e % 4;
-        lds[o][0][r * 4 + (c ^ (r / 2 % 4))] = next[o][0][l];
-        lds[o][1][r * 4 + (c ^ (r / 2 % 4))] = next[o][1][l];
-      }
-    __syncthreads();
-    if (k + 32 < pr.k) fetch(k + 32);
+  for (int p = 0; p < BUFFERS - 1; ++p)
+    if (p < steps) fetch(p, p);
+  int buffer = 0;
+  for (int step = 0; step < steps; ++step) {
+    // This step's pieces have come (a wave's loads come in order, 4 LOADS a
+    // step, and those of BUFFERS - 2 later steps may still be under way), this
+    // wave's reads of the step before are done, and so are everybody's.
+    if (step + BUFFERS - 1 <= steps)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier"
+                   :: "n"((BUFFERS - 2) * 4 * LOADS) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (step + BUFFERS - 1 < steps)
+      fetch(step + BUFFERS - 1,
+            buffer ? buffer - 1 : BUFFERS - 1);
     half8 av[W][2], bv[W][2];
 #pragma unroll
     for (int t = 0; t < W; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        int ra = wi + t * 16 + lane % 16, rb = wj + t * 16 + lane % 16;
-        av[t][h] = lds[0][h][ra * 4 + (lane / 16 ^ (ra / 2 % 4))];
-        bv[t][h] = lds[1][h][rb * 4 + (lane / 16 ^ (rb / 2 % 4))];
+        const int ra = wi + t * 16 + lane % 16, rb = wj + t * 16 + lane % 16;
+        av[t][h] = lds[buffer][0][h][ra * 4 + (lane / 16 ^ (ra / 2 % 4))];
+        bv[t][h] = lds[buffer][1][h][rb * 4 + (lane / 16 ^ (rb / 2 % 4))];
       }
 #pragma unroll
     for (int i = 0; i < W; ++i)
@@ -1065,51 +1213,46 @@ __global__ __launch_bounds__(256) void k_product(
         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
             av[i][0], bv[j][0], acc[i][j], 0, 0, 0);
       }
+    buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
   }
 
-  // a lane holds D[i .. i + 3][j] of each tile
+  if (shared) {
 #pragma unroll
-  for (int ti = 0; ti < W; ++ti)
+    for (int i = 0; i < W; ++i)
 #pragma unroll
-    for (int tj = 0; tj < W; ++tj) {
-      const int64_t i = (int64_t)bi * NT + wi + ti * 16 + lane / 16 * 4;
-      const int64_t j = (int64_t)bj * NT + wj + tj * 16 + lane % 16;
-      if (E == FINAL) {
+      for (int j = 0; j < W; ++j)
+        ((f32x4*)parts)[(i * W + j) * 256 + threadIdx.x] = acc[i][j];
+    return;
+  }
+  end_product<NT, E, T>(pr, b, bi, bj, acc, (_Float16*)lds);
+}
+
+// The tiles whose sum was shared out: its parts, in their order.
+template <int NT, Ending E, typename T>
+__global__ __launch_bounds__(256) void k_join(
+    Product pr, const int* __restrict__ touched) {
+  constexpr int W = NT / 32;
+  __shared__ half8 lds[NT * (NT + 8) / 8];
+  const int64_t tile = pr.whole + blockIdx.x;
+  const int64_t b = tile / pr.tiles;
+  if (touched && !touched[b]) return;
+  int bi, bj;
+  tile_of<E == GRAM || E == POLY>(tile % pr.tiles, pr.ns, pr.nl, &bi, &bj);
+  const f32x4* parts = (const f32x4*)pr.parts +
+                       (int64_t)blockIdx.x * pr.splits * (W * W * 256);
+  f32x4 acc[W][W];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (i + r < pr.rows && j < pr.cols)
-            finish<T>(pr.res,
-                      b * pr.rows * pr.cols +
-                          (pr.tall ? j * pr.rows + i + r
-                                   : (i + r) * pr.cols + j),
-                      acc[ti][tj][r] * (1.0f / (UP * UP)));
-        continue;
-      }
-      half4 hi, lo;
+  for (int i = 0; i < W; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float v = acc[ti][tj][r] * (1.0f / UP);
-        if (E == POLY) {
-          const _Float16* g = pr.a.p + b * pr.a.batch +
-                              (i + r) * pr.a.pitch + j;
-          v = pr.cc * v + pr.cb * ((float)g[0] + (float)g[pr.a.plane]);
-          if (i + r == j && j < pr.s) v += pr.ca * UP;
-        }
-        _Float16 h, l;
-        split(v, h, l);
-        hi[r] = h;
-        lo[r] = l;
-        _Float16* to = pr.d.p + b * pr.d.batch + (i + r) * pr.d.pitch + j;
-        to[0] = h;
-        to[pr.d.plane] = l;
-      }
-      if (E == UPDATE || bi != bj) {
-        const Planes& t = E == UPDATE ? pr.dt : pr.d;
-        _Float16* to = t.p + b * t.batch + j * t.pitch + i;
-        *(half4*)to = hi;
-        *(half4*)(to + t.plane) = lo;
-      }
-    }
+    for (int j = 0; j < W; ++j) acc[i][j] = parts[(i * W + j) * 256 +
+                                                  threadIdx.x];
+  for (int q = 1; q < pr.splits; ++q)
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        acc[i][j] += parts[((q * W + i) * W + j) * 256 + threadIdx.x];
+  end_product<NT, E, T>(pr, b, bi, bj, acc, (_Float16*)lds);
 }
 
 // ---------------------------------------------------------------------
@@ -1235,45 +1378,57 @@ void run_thin(const Chain& c) {
   else apply(k_thin_apply<T, TALL, 8, 128>);
 }
 
-template <int NT, typename T>
-void run_products(const Chain& c, Planes x, Planes xt, Planes xt2, Planes g,
-                  Planes q) {
-  const int64_t s = std::min(c.m, c.n), long_ = std::max(c.m, c.n);
-  const int ns = (s + NT - 1) / NT, nl = (long_ + NT - 1) / NT;
-  const dim3 half(ns * (ns + 1) / 2, 1, c.batch), full(nl, ns, c.batch);
-  Product pr{};
-  pr.ca = (float)c.k.a;
-  pr.cb = (float)c.k.b;
-  pr.cc = (float)c.k.c;
-  pr.s = s;
-  pr.rows = s;
-  pr.cols = long_;
-  pr.tall = c.m > c.n;
-  pr.res = c.res;
-  const int ks = round_up(s, 32), kl = round_up(long_, 32);
-  for (int i = 0; i < c.steps; ++i) {
-    pr.a = pr.b = x;
-    pr.k = kl;
-    pr.d = g;
-    hipLaunchKernelGGL((k_product<NT, GRAM, T>), half, dim3(256), 0, c.stream,
-                       pr, c.touched);
-    pr.a = pr.b = g;
-    pr.k = ks;
-    pr.d = q;
-    hipLaunchKernelGGL((k_product<NT, POLY, T>), half, dim3(256), 0, c.stream,
-                       pr, c.touched);
-    pr.a = q;
-    pr.b = xt;
-    pr.d = x;
-    pr.dt = xt2;
-    if (i + 1 < c.steps)
-      hipLaunchKernelGGL((k_product<NT, UPDATE, T>), full, dim3(256), 0,
-                         c.stream, pr, c.touched);
-    else
-      hipLaunchKernelGGL((k_product<NT, FINAL, T>), full, dim3(256), 0,
-                         c.stream, pr, c.touched);
-    std::swap(xt, xt2);
+// Tiles of one product, and how many blocks share the sum of those after the
+// first `whole`.
+struct Cut {
+  int tile, ns, nl, tiles, splits;
+  int64_t all, whole;
+};
+
+// 128 x 128 tiles where they give every CU one, else 64 x 64.  Two blocks fit
+// a CU: tiles that are left over after a number of full rounds would keep the
+// card for a round of their own, so their sums are shared out, as are those of
+// all tiles where there are too few.  A share is 16 steps of 32 places at
+// least: what the join costs is about that.
+Cut cut_of(int64_t rows, int64_t cols, bool half, int64_t batch, int64_t k) {
+  constexpr int64_t ROUND = 512;
+  Cut c{};
+  for (c.tile = 128;; c.tile = 64) {
+    c.ns = (rows + c.tile - 1) / c.tile;
+    c.nl = (cols + c.tile - 1) / c.tile;
+    c.tiles = half ? c.ns * (c.ns + 1) / 2 : c.ns * c.nl;
+    c.all = c.tiles * batch;
+    if (c.tile == 64 || c.all >= ROUND / 2) break;
   }
+  const int64_t rest = c.all % ROUND, steps = round_up(k, 32) / 32;
+  c.splits = 1;
+  c.whole = c.all;
+  if (rest && rest <= ROUND / 2 && c.all < 8 * ROUND && steps >= 32) {
+    c.splits = std::min(ROUND / rest, steps / 16);
+    c.whole = c.all - rest;
+  }
+  return c;
+}
+
+template <Ending E, typename T>
+void run_product(const Chain& c, Product pr, const Cut& cut) {
+  pr.ns = cut.ns;
+  pr.nl = cut.nl;
+  pr.tiles = cut.tiles;
+  pr.all = cut.all;
+  pr.whole = cut.whole;
+  pr.splits = cut.splits;
+  const int64_t rest = cut.all - cut.whole;
+  const dim3 grid(round_up(cut.whole, XCDS) +
+                  round_up(rest * cut.splits, XCDS));
+  auto go = [&](auto* kfn, auto* join) {
+    hipLaunchKernelGGL(kfn, grid, dim3(256), 0, c.stream, pr, c.touched);
+    if (rest)
+      hipLaunchKernelGGL(join, dim3(rest), dim3(256), 0, c.stream, pr,
+                         c.touched);
+  };
+  if (cut.tile == 128) go(k_product<128, 2, E, T>, k_join<128, E, T>);
+  else go(k_product<64, 4, E, T>, k_join<64, E, T>);
 }
 
 template <typename T>
@@ -1293,20 +1448,52 @@ void run_wide(const Chain& c) {
   Planes xt2 = tall ? planes(mp, np) : planes(np, mp);
   Planes g = planes(sp, sp), q = planes(sp, sp);
   const int parts = (int)std::min<int64_t>(
-      256, (c.m * c.n + 4095) / 4096);
+      std::max<int64_t>(1, 1024 / c.batch), (c.m * c.n + 4095) / 4096);
   auto part = at::empty({c.batch * parts}, c.options.dtype(at::kDouble));
-  auto scale = at::empty({2 * c.batch}, c.options.dtype(at::kFloat));
   hipLaunchKernelGGL(k_sumsq<T>, dim3(parts, c.batch), dim3(256), 0, c.stream,
                      part.data_ptr<double>(), (const T*)c.u, c.touched,
                      c.m * c.n);
-  hipLaunchKernelGGL(k_norm, dim3((c.batch + 255) / 256), dim3(256), 0,
-                     c.stream, (float2*)scale.data_ptr<float>(),
-                     part.data_ptr<double>(), parts, c.batch, c.eps);
   hipLaunchKernelGGL(k_planes<T>, dim3(np / 64 * (mp / 64), 1, c.batch),
                      dim3(256), 0, c.stream, nat, trn, (const T*)c.u,
-                     (const float2*)scale.data_ptr<float>(), c.touched, c.m,
-                     c.n);
-  run_products<64, T>(c, x, xt, xt2, g, q);
+                     part.data_ptr<double>(), parts, c.touched, c.m, c.n,
+                     c.eps);
+  const int64_t long_ = std::max(c.m, c.n);
+  const Cut gram = cut_of(s, s, true, c.batch, long_);
+  const Cut poly = cut_of(s, s, true, c.batch, s);
+  const Cut full = cut_of(s, long_, false, c.batch, s);
+  int64_t shared = 0;
+  for (const Cut& cut : {gram, poly, full})
+    shared = std::max(shared, (cut.all - cut.whole) * cut.splits * cut.tile *
+                                  cut.tile);
+  auto sums = at::empty({shared}, c.options.dtype(at::kFloat));
+  Product pr{};
+  pr.ca = (float)c.k.a;
+  pr.cb = (float)c.k.b;
+  pr.cc = (float)c.k.c;
+  pr.s = s;
+  pr.rows = s;
+  pr.cols = long_;
+  pr.tall = tall;
+  pr.res = c.res;
+  pr.parts = sums.data_ptr<float>();
+  const int ks = round_up(s, 32), kl = round_up(long_, 32);
+  for (int i = 0; i < c.steps; ++i) {
+    pr.a = pr.b = x;
+    pr.k = kl;
+    pr.d = g;
+    run_product<GRAM, T>(c, pr, gram);
+    pr.a = pr.b = g;
+    pr.k = ks;
+    pr.d = q;
+    run_product<POLY, T>(c, pr, poly);
+    pr.a = q;
+    pr.b = xt;
+    pr.d = x;
+    pr.dt = xt2;
+    if (i + 1 < c.steps) run_product<UPDATE, T>(c, pr, full);
+    else run_product<FINAL, T>(c, pr, full);
+    std::swap(xt, xt2);
+  }
 }
 
 template <typename T>
