@@ -43,6 +43,11 @@ using f64x4 = __attribute__((ext_vector_type(4))) double;
 
 struct Coeffs { double a, b, c; };
 
+template <typename I>
+__host__ __device__ inline I round_up(I v, int to) {
+  return (v + to - 1) / to * to;
+}
+
 // What a product ends in: the values of `out` (T), or the weights' step
 // W <- W keep - rate O.
 struct Result {
@@ -179,6 +184,29 @@ __global__ __launch_bounds__(256) void k_places(
                                : (order ? order[j] : j);
   __syncthreads();
   if (threadIdx.x < count) place[r0 + threadIdx.x] = mine[threadIdx.x];
+}
+
+// active[0] = how many of up to 32768 matrices are touched, then which.
+__global__ __launch_bounds__(1024) void k_active(
+    int* __restrict__ active, const int* __restrict__ touched, int batch) {
+  __shared__ int counts[16];
+  int before = 0;
+  for (int b0 = 0; b0 < batch; b0 += 1024) {
+    const int b = b0 + threadIdx.x;
+    const bool mine = b < batch && touched[b];
+    const uint64_t votes = __ballot(mine);
+    const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
+    if (lane == 0) counts[wave] = __popcll(votes);
+    __syncthreads();
+    int at = before;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) at += counts[w];
+      before += counts[w];
+    }
+    if (mine) active[1 + at + __popcll(votes & ((1ull << lane) - 1))] = b;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) active[0] = before;
 }
 
 // M <- mu M + g and U = g + mu M (nesterov) or M, `group` lanes a row.  Bound
@@ -980,7 +1008,7 @@ struct Product {
   // of all tiles the first `whole` are a block's each, the others have their
   // sum shared out to `splits` blocks, which leave it in `parts`
   int ns, nl, tiles, splits;
-  int64_t all, whole;
+  uint32_t all, whole;
   float* parts;
 };
 
@@ -1111,38 +1139,50 @@ __device__ inline void end_product(const Product& pr, int64_t b, int bi,
 // 16 x 16 x 32 operands.
 template <int NT, int BUFFERS, Ending E, typename T>
 __global__ __launch_bounds__(256, 2) void k_product(
-    Product pr, const int* __restrict__ touched) {
+    Product pr, const int* __restrict__ active) {
   constexpr bool HALF = E == GRAM || E == POLY;
   constexpr int W = NT / 32;           // 16-tiles a wave on each side
   constexpr int LOADS = NT / 64;       // pieces a thread, operand and plane
   __shared__ half8 lds[BUFFERS][2][2][NT * 4];  // buffer, operand, plane
   static_assert(NT * (NT + 8) * sizeof(_Float16) <= sizeof(lds), "");
 
-  // each XCD takes one run of the whole tiles, and one of the shares
-  int64_t id = blockIdx.x, count = pr.whole, tile;
-  int part = 0, splits = 1;
-  const bool shared = id >= (pr.whole + XCDS - 1) / XCDS * XCDS;
+  // each XCD takes one run of the whole tiles of the matrices there are to do,
+  // and one of the shares (32 bits: divisions by 64 cost as much as a step)
+  uint32_t id = blockIdx.x, count = pr.whole, splits = 1;
+  const uint32_t shares = round_up((uint32_t)pr.whole, XCDS);
+  const bool shared = id >= shares;
   if (shared) {
-    id -= (pr.whole + XCDS - 1) / XCDS * XCDS;
+    id -= shares;
     splits = pr.splits;
     count = (pr.all - pr.whole) * splits;
+  } else if (active) {
+    count = min(count, (uint32_t)(active[0] * pr.tiles));
   }
-  const int64_t each = (count + XCDS - 1) / XCDS;
+  const uint32_t each = (count + XCDS - 1) / XCDS;
+  if (id / XCDS >= each) return;
   id = id % XCDS * each + id / XCDS;
   if (id >= count) return;
-  tile = id / splits;
-  part = id % splits;
-  float* parts = pr.parts + id * (NT * NT);
-  if (shared) tile += pr.whole;
-  const int64_t b = tile / pr.tiles;
-  if (touched && !touched[b]) return;
+  float* parts = pr.parts + (int64_t)id * (NT * NT);
+  uint32_t tile = id, part = 0;
+  if (shared) {
+    tile = id / splits;
+    part = id - tile * splits;
+    tile += pr.whole;
+  }
+  const uint32_t matrix = tile / (uint32_t)pr.tiles;
+  if (active && matrix >= (uint32_t)active[0]) return;
+  const int64_t b = active ? active[1 + matrix] : matrix;
   int bi, bj;
-  tile_of<HALF>(tile % pr.tiles, pr.ns, pr.nl, &bi, &bj);
+  tile_of<HALF>(tile - matrix * pr.tiles, pr.ns, pr.nl, &bi, &bj);
 
   const int lane = threadIdx.x % WAVE, wave = this_wave();
   const int wi = wave / 2 * (NT / 2), wj = wave % 2 * (NT / 2);
-  const int first = (int64_t)(pr.k / 32) * part / splits;
-  const int steps = (int)((int64_t)(pr.k / 32) * (part + 1) / splits) - first;
+  int first = 0, steps = pr.k / 32;
+  if (shared) {
+    const uint32_t share = steps / splits, more = steps - share * splits;
+    first = part * share + min(part, more);
+    steps = share + (part < more);
+  }
 
   const _Float16* src[2] = {
       pr.a.p + b * pr.a.batch + (int64_t)bi * NT * pr.a.pitch + first * 32,
@@ -1190,9 +1230,6 @@ __global__ __launch_bounds__(256, 2) void k_product(
                    :: "n"((BUFFERS - 2) * 4 * LOADS) : "memory");
     else
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (step + BUFFERS - 1 < steps)
-      fetch(step + BUFFERS - 1,
-            buffer ? buffer - 1 : BUFFERS - 1);
     half8 av[W][2], bv[W][2];
 #pragma unroll
     for (int t = 0; t < W; ++t)
@@ -1202,6 +1239,9 @@ __global__ __launch_bounds__(256, 2) void k_product(
         av[t][h] = lds[buffer][0][h][ra * 4 + (lane / 16 ^ (ra / 2 % 4))];
         bv[t][h] = lds[buffer][1][h][rb * 4 + (lane / 16 ^ (rb / 2 % 4))];
       }
+    if (step + BUFFERS - 1 < steps)
+      fetch(step + BUFFERS - 1,
+            buffer ? buffer - 1 : BUFFERS - 1);
 #pragma unroll
     for (int i = 0; i < W; ++i)
 #pragma unroll
@@ -1230,14 +1270,16 @@ __global__ __launch_bounds__(256, 2) void k_product(
 // The tiles whose sum was shared out: its parts, in their order.
 template <int NT, Ending E, typename T>
 __global__ __launch_bounds__(256) void k_join(
-    Product pr, const int* __restrict__ touched) {
+    Product pr, const int* __restrict__ active) {
   constexpr int W = NT / 32;
   __shared__ half8 lds[NT * (NT + 8) / 8];
-  const int64_t tile = pr.whole + blockIdx.x;
-  const int64_t b = tile / pr.tiles;
-  if (touched && !touched[b]) return;
+  const uint32_t tile = pr.whole + blockIdx.x;
+  const uint32_t matrix = tile / (uint32_t)pr.tiles;
+  if (active && matrix >= (uint32_t)active[0]) return;
+  const int64_t b = active ? active[1 + matrix] : matrix;
   int bi, bj;
-  tile_of<E == GRAM || E == POLY>(tile % pr.tiles, pr.ns, pr.nl, &bi, &bj);
+  tile_of<E == GRAM || E == POLY>(tile - matrix * pr.tiles, pr.ns, pr.nl, &bi,
+                                  &bj);
   const f32x4* parts = (const f32x4*)pr.parts +
                        (int64_t)blockIdx.x * pr.splits * (W * W * 256);
   f32x4 acc[W][W];
@@ -1264,6 +1306,7 @@ struct Chain {
   at::ScalarType type;
   int64_t batch, m, n;
   const int* touched;
+  const int* active;  // how many are touched, and which
   int steps;
   Coeffs k;
   double eps;
@@ -1282,7 +1325,6 @@ bool is_thin(int64_t m, int64_t n) {
   return s <= NARROW || (s <= THIN_MAX && long_ >= 32 * s);
 }
 
-int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 template <typename T, bool TALL>
 void run_thin(const Chain& c) {
@@ -1388,8 +1430,8 @@ struct Cut {
 // 128 x 128 tiles where they give every CU one, else 64 x 64.  Two blocks fit
 // a CU: tiles that are left over after a number of full rounds would keep the
 // card for a round of their own, so their sums are shared out, as are those of
-// all tiles where there are too few.  A share is 16 steps of 32 places at
-// least: what the join costs is about that.
+// all tiles where there are too few.  A share is `least` steps of 32 places:
+// what the join costs is about that.
 Cut cut_of(int64_t rows, int64_t cols, bool half, int64_t batch, int64_t k) {
   constexpr int64_t ROUND = 512;
   Cut c{};
@@ -1400,11 +1442,12 @@ Cut cut_of(int64_t rows, int64_t cols, bool half, int64_t batch, int64_t k) {
     c.all = c.tiles * batch;
     if (c.tile == 64 || c.all >= ROUND / 2) break;
   }
+  const int64_t least = c.tile == 128 ? 16 : 32;
   const int64_t rest = c.all % ROUND, steps = round_up(k, 32) / 32;
   c.splits = 1;
   c.whole = c.all;
-  if (rest && rest <= ROUND / 2 && c.all < 8 * ROUND && steps >= 32) {
-    c.splits = std::min(ROUND / rest, steps / 16);
+  if (rest && rest <= ROUND / 2 && c.all < 8 * ROUND && steps >= 2 * least) {
+    c.splits = std::min(ROUND / rest, steps / least);
     c.whole = c.all - rest;
   }
   return c;
@@ -1422,10 +1465,10 @@ void run_product(const Chain& c, Product pr, const Cut& cut) {
   const dim3 grid(round_up(cut.whole, XCDS) +
                   round_up(rest * cut.splits, XCDS));
   auto go = [&](auto* kfn, auto* join) {
-    hipLaunchKernelGGL(kfn, grid, dim3(256), 0, c.stream, pr, c.touched);
+    hipLaunchKernelGGL(kfn, grid, dim3(256), 0, c.stream, pr, c.active);
     if (rest)
       hipLaunchKernelGGL(join, dim3(rest), dim3(256), 0, c.stream, pr,
-                         c.touched);
+                         c.active);
   };
   if (cut.tile == 128) go(k_product<128, 2, E, T>, k_join<128, E, T>);
   else go(k_product<64, 4, E, T>, k_join<64, E, T>);
@@ -1514,7 +1557,16 @@ void dispatch(const Chain& whole) {
     c.u = (const char*)c.u + size * c10::elementSize(c.type);
     c.res.out = (char*)c.res.out +
                 size * (c.res.step ? 4 : c10::elementSize(c.type));
-    if (c.touched) c.touched += b;
+    at::Tensor active;
+    if (c.touched) {
+      c.touched += b;
+      if (!is_thin(c.m, c.n)) {
+        active = at::empty({c.batch + 1}, c.options.dtype(at::kInt));
+        c.active = active.data_ptr<int>();
+        hipLaunchKernelGGL(k_active, dim3(1), dim3(1024), 0, c.stream,
+                           active.data_ptr<int>(), c.touched, (int)c.batch);
+      }
+    }
     if (c.type == at::kFloat) run<float>(c);
     else if (c.type == at::kHalf) run<__half>(c);
     else run<__hip_bfloat16>(c);
@@ -1542,7 +1594,7 @@ at::Tensor orthogonalize(at::Tensor x, int64_t steps, double a, double b,
   auto out = at::empty_like(x);
   if (!x.numel()) return out;
   dispatch(Chain{x.data_ptr(), type, x.size(0), x.size(1), x.size(2), nullptr,
-                 (int)steps, {a, b, c}, eps, {out.data_ptr(), 0, 0, false},
+                 nullptr, (int)steps, {a, b, c}, eps, {out.data_ptr(), 0, 0, false},
                  x.options(), at::hip::getCurrentHIPStream().stream()});
   return out;
 }
@@ -1606,7 +1658,7 @@ void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
   }
   const double rate = lr * std::sqrt(std::max(1.0, (double)matrix_rows / dim));
   Chain chain{u.data_ptr(), at::kFloat, batch, matrix_rows, dim,
-              touched.data_ptr<int>(), (int)steps, {a, b, c}, eps,
+              touched.data_ptr<int>(), nullptr, (int)steps, {a, b, c}, eps,
               {table.data_ptr(), (float)(1.0 - lr * weight_decay),
                (float)rate, true},
               table.options(), stream};

@@ -7,6 +7,7 @@ in-tree extension; a missing extension raises (never a silent fallback).
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -231,9 +232,25 @@ def _check_chain(name: str, steps: int, coeffs: Sequence[float],
     if not 0 < eps < float("inf"):
         raise ValueError(f"{name}: eps must be positive, got {eps}")
     a, b, c = (float(v) for v in coeffs)
-    if abs(a) > 12 or abs(b) > 12 or abs(c) > 12:
-        raise ValueError(f"{name}: coefficients beyond 12, got {coeffs!r}")
+    if not _bounded(a, b, c, int(steps)):
+        raise ValueError(f"{name}: with coeffs {coeffs!r} singular values "
+                         f"grow beyond 3.9 in {steps} steps")
     return a, b, c
+
+
+@lru_cache(maxsize=64)
+def _bounded(a: float, b: float, c: float, steps: int) -> bool:
+    """Whether singular values from [0, 1] stay within 3.9, and what a step
+    multiplies them by within 15.9: the kernels hold values in f16 planes
+    scaled by 2^12."""
+    x = torch.linspace(0.0, 1.0, 4097, dtype=torch.float64)
+    for _ in range(steps):
+        q = a + b * x ** 2 + c * x ** 4
+        x = q * x
+        if not (bool((x.abs() <= 3.9).all()) and
+                bool((q.abs() <= 15.9).all())):
+            return False
+    return True
 
 
 def orthogonalize(x: torch.Tensor, steps: int = 5,

@@ -190,7 +190,11 @@ def test_orthogonalize_refusals(device):
                 lambda: ops.orthogonalize(x, eps=0.0),
                 lambda: ops.orthogonalize(x, eps=float("nan")),
                 lambda: ops.orthogonalize(x, coeffs=(1.0, 2.0)),
-                lambda: ops.orthogonalize(x, coeffs=(1.0, float("inf"), 0))):
+                lambda: ops.orthogonalize(x, coeffs=(1.0, float("inf"), 0)),
+                lambda: ops.orthogonalize(x, coeffs=(1.0, float("nan"), 0)),
+                lambda: ops.orthogonalize(x, coeffs=(2.0, 0.0, 0.0)),
+                lambda: ops.orthogonalize(x, coeffs=(16.0, -20.0, 0.0),
+                                          steps=1)):
         with pytest.raises(ValueError):
             bad()
     with pytest.raises(RuntimeError):
