@@ -995,10 +995,16 @@ __global__ __launch_bounds__(256) void k_planes(
 
 enum Ending { GRAM, POLY, UPDATE, FINAL };
 
+// D[i][j] = scale sum_k a[i][k] b[j][k], of the values that the planes hold.
+struct Factors {
+  Planes a, b, d;
+  float scale;
+};
+
 struct Product {
-  Planes a, b;       // rows of K values each: D[i][j] = sum_k a[i][k] b[j][k]
+  Factors f[2];      // blockIdx.y says which
   int k;             // a multiple of 32
-  Planes d, dt;      // D and D transposed (GRAM, POLY: d alone, symmetric)
+  Planes dt;         // UPDATE: D transposed (GRAM, POLY: D is symmetric)
   float ca, cb, cc;  // POLY: a I + b a + c D
   int s;             // POLY: I ends here
   int64_t rows, cols;  // FINAL: D's own size
@@ -1051,8 +1057,9 @@ __device__ inline void tile_of(int t, int ns, int nl, int* bi, int* bj) {
 // What one block leaves of its tile: a lane holds D[i .. i + 3][j] of each
 // 16 x 16 tile of its wave's quarter.  `lds` is free to be written.
 template <int NT, Ending E, typename T>
-__device__ inline void end_product(const Product& pr, int64_t b, int bi,
-                                   int bj, f32x4 (&acc)[NT / 32][NT / 32],
+__device__ inline void end_product(const Product& pr, const Factors& f,
+                                   int64_t b, int bi, int bj,
+                                   f32x4 (&acc)[NT / 32][NT / 32],
                                    _Float16* lds) {
   constexpr int W = NT / 32;
   const int lane = threadIdx.x % WAVE, wave = this_wave();
@@ -1065,7 +1072,7 @@ __device__ inline void end_product(const Product& pr, int64_t b, int bi,
         const int64_t i = (int64_t)bi * NT + wi + ti * 16 + lane / 16 * 4;
         const int64_t j = (int64_t)bj * NT + wj + tj * 16 + lane % 16;
         if (j >= pr.cols) continue;
-        const f32x4 v = acc[ti][tj] * (1.0f / (UP * UP));
+        const f32x4 v = acc[ti][tj] * f.scale;
         const int64_t base = b * pr.rows * pr.cols;
         if (pr.tall) {
           finish_quad<T>(pr.res, base + j * pr.rows + i,
@@ -1093,12 +1100,12 @@ __device__ inline void end_product(const Product& pr, int64_t b, int bi,
         const int lj = wj + tj * 16 + lane % 16;
         const int64_t i = (int64_t)bi * NT + li, j = (int64_t)bj * NT + lj;
         if (h == 0) {
-          f32x4 v = acc[ti][tj] * (1.0f / UP);
+          f32x4 v = acc[ti][tj] * f.scale;
           if (E == POLY) {
             // a is symmetric: its row j has the four values side by side
-            const _Float16* g = pr.a.p + b * pr.a.batch + j * pr.a.pitch + i;
+            const _Float16* g = f.a.p + b * f.a.batch + j * f.a.pitch + i;
             const half4 gh = *(const half4*)g;
-            const half4 gl = *(const half4*)(g + pr.a.plane);
+            const half4 gl = *(const half4*)(g + f.a.plane);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               v[r] = pr.cc * v[r] + pr.cb * ((float)gh[r] + (float)gl[r]);
@@ -1116,15 +1123,15 @@ __device__ inline void end_product(const Product& pr, int64_t b, int bi,
           lds[(li + r) * ROW + lj] = w[r];
         }
         if (E == UPDATE || bi != bj) {
-          const Planes& t = E == UPDATE ? pr.dt : pr.d;
+          const Planes& t = E == UPDATE ? pr.dt : f.d;
           *(half4*)(t.p + h * t.plane + b * t.batch + j * t.pitch + i) = w;
         }
       }
     __syncthreads();
     for (int e = threadIdx.x; e < NT * NT / 8; e += 256) {
       const int r = e / (NT / 8), c = e % (NT / 8) * 8;
-      *(half8*)(pr.d.p + h * pr.d.plane + b * pr.d.batch +
-                ((int64_t)bi * NT + r) * pr.d.pitch + (int64_t)bj * NT + c) =
+      *(half8*)(f.d.p + h * f.d.plane + b * f.d.batch +
+                ((int64_t)bi * NT + r) * f.d.pitch + (int64_t)bj * NT + c) =
           *(const half8*)(lds + r * ROW + c);
     }
   }
@@ -1162,7 +1169,8 @@ __global__ __launch_bounds__(256, 2) void k_product(
   if (id / XCDS >= each) return;
   id = id % XCDS * each + id / XCDS;
   if (id >= count) return;
-  float* parts = pr.parts + (int64_t)id * (NT * NT);
+  float* parts = pr.parts + (blockIdx.y * (int64_t)(pr.all - pr.whole) *
+                                 pr.splits + id) * (NT * NT);
   uint32_t tile = id, part = 0;
   if (shared) {
     tile = id / splits;
@@ -1184,17 +1192,18 @@ __global__ __launch_bounds__(256, 2) void k_product(
     steps = share + (part < more);
   }
 
+  const Factors f = HALF && blockIdx.y ? pr.f[1] : pr.f[0];
   const _Float16* src[2] = {
-      pr.a.p + b * pr.a.batch + (int64_t)bi * NT * pr.a.pitch + first * 32,
-      pr.b.p + b * pr.b.batch + (int64_t)bj * NT * pr.b.pitch + first * 32};
-  const int64_t plane[2] = {pr.a.plane, pr.b.plane};
+      f.a.p + b * f.a.batch + (int64_t)bi * NT * f.a.pitch + first * 32,
+      f.b.p + b * f.b.batch + (int64_t)bj * NT * f.b.pitch + first * 32};
+  const int64_t plane[2] = {f.a.plane, f.b.plane};
   int64_t from[2][LOADS];
 #pragma unroll
   for (int l = 0; l < LOADS; ++l) {
     const int e = (l * 4 + wave) * WAVE + lane, r = e / 4;
     const int c = (e % 4 ^ (r / 2 % 4)) * 8;
-    from[0][l] = r * pr.a.pitch + c;
-    from[1][l] = r * pr.b.pitch + c;
+    from[0][l] = r * f.a.pitch + c;
+    from[1][l] = r * f.b.pitch + c;
   }
   auto fetch = [&](int step, int buffer) {
 #pragma unroll
@@ -1264,7 +1273,7 @@ __global__ __launch_bounds__(256, 2) void k_product(
         ((f32x4*)parts)[(i * W + j) * 256 + threadIdx.x] = acc[i][j];
     return;
   }
-  end_product<NT, E, T>(pr, b, bi, bj, acc, (_Float16*)lds);
+  end_product<NT, E, T>(pr, f, b, bi, bj, acc, (_Float16*)lds);
 }
 
 // The tiles whose sum was shared out: its parts, in their order.
@@ -1280,8 +1289,10 @@ __global__ __launch_bounds__(256) void k_join(
   int bi, bj;
   tile_of<E == GRAM || E == POLY>(tile - matrix * pr.tiles, pr.ns, pr.nl, &bi,
                                   &bj);
+  const Factors& f = pr.f[blockIdx.y];
   const f32x4* parts = (const f32x4*)pr.parts +
-                       (int64_t)blockIdx.x * pr.splits * (W * W * 256);
+                       ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) *
+                           pr.splits * (W * W * 256);
   f32x4 acc[W][W];
 #pragma unroll
   for (int i = 0; i < W; ++i)
@@ -1294,7 +1305,7 @@ __global__ __launch_bounds__(256) void k_join(
 #pragma unroll
       for (int j = 0; j < W; ++j)
         acc[i][j] += parts[((q * W + i) * W + j) * 256 + threadIdx.x];
-  end_product<NT, E, T>(pr, b, bi, bj, acc, (_Float16*)lds);
+  end_product<NT, E, T>(pr, f, b, bi, bj, acc, (_Float16*)lds);
 }
 
 // ---------------------------------------------------------------------
@@ -1320,9 +1331,12 @@ struct Chain {
   const int64_t* place = nullptr;
 };
 
-bool is_thin(int64_t m, int64_t n) {
+bool is_thin(int64_t batch, int64_t m, int64_t n) {
   const int64_t s = std::min(m, n), long_ = std::max(m, n);
-  return s <= NARROW || (s <= THIN_MAX && long_ >= 32 * s);
+  // measured, thin against wide: 1 x 128 x 2048 95 us, 139; 4 x 128 x 512 107,
+  // 109; 16 x 128 x 512 163, 110; 256 x 4096 177, 178; 320 x 5000 249, 224
+  return s <= NARROW || (s <= THIN_MAX && long_ >= 32 * s) ||
+         (s <= SUPER && long_ >= 4 * s && batch * s <= 4 * SUPER);
 }
 
 
@@ -1454,7 +1468,7 @@ Cut cut_of(int64_t rows, int64_t cols, bool half, int64_t batch, int64_t k) {
 }
 
 template <Ending E, typename T>
-void run_product(const Chain& c, Product pr, const Cut& cut) {
+void run_product(const Chain& c, Product pr, const Cut& cut, int jobs = 1) {
   pr.ns = cut.ns;
   pr.nl = cut.nl;
   pr.tiles = cut.tiles;
@@ -1463,15 +1477,53 @@ void run_product(const Chain& c, Product pr, const Cut& cut) {
   pr.splits = cut.splits;
   const int64_t rest = cut.all - cut.whole;
   const dim3 grid(round_up(cut.whole, XCDS) +
-                  round_up(rest * cut.splits, XCDS));
+                      round_up(rest * cut.splits, XCDS),
+                  jobs);
   auto go = [&](auto* kfn, auto* join) {
     hipLaunchKernelGGL(kfn, grid, dim3(256), 0, c.stream, pr, c.active);
     if (rest)
-      hipLaunchKernelGGL(join, dim3(rest), dim3(256), 0, c.stream, pr,
+      hipLaunchKernelGGL(join, dim3(rest, jobs), dim3(256), 0, c.stream, pr,
                          c.active);
   };
   if (cut.tile == 128) go(k_product<128, 2, E, T>, k_join<128, E, T>);
   else go(k_product<64, 4, E, T>, k_join<64, E, T>);
+}
+
+// How far P's values can reach: its value at singular values from 0 to 1.
+struct Reach {
+  double x[257], p[257];
+  Reach() {
+    for (int i = 0; i < 257; ++i) {
+      x[i] = i / 256.0;
+      p[i] = 1.0;
+    }
+  }
+  void step(const Coeffs& k) {
+    for (int i = 0; i < 257; ++i) {
+      const double y = x[i] * x[i], q = k.a + k.b * y + k.c * y * y;
+      p[i] *= q;
+      x[i] *= q;
+    }
+  }
+  // the power of two that keeps P under 4, up to what lies between the points
+  float hold() const {
+    double top = 0;
+    for (double v : p) top = std::max(top, std::abs(v));
+    return top > 4 ? (float)std::exp2(-std::ceil(std::log2(top / 4))) : 1.0f;
+  }
+};
+
+// Whether all steps are taken on the Gram matrix, before P is applied to X.
+// With L = r s a step costs 3 r + 1 products of s^3 on X and about 4 on s x s
+// matrices, which need 3 r for G and P X once.  What G is off grows by a^2 with
+// every step and reaches a few parts in 10^4 of the result after five of Muon's:
+// below bfloat16's rounding, not below the others'; with more steps, which bring
+// up smaller singular values, it does not stay there.
+template <typename T>
+bool by_gram(const Chain& c, int64_t s, int64_t long_) {
+  return std::is_same_v<T, __hip_bfloat16> && c.steps > 1 &&
+         long_ * 2 >= s * 3 &&
+         std::pow(c.k.a * c.k.a, c.steps - 1) <= 21000.0;
 }
 
 template <typename T>
@@ -1488,8 +1540,6 @@ void run_wide(const Chain& c) {
   };
   Planes nat = planes(mp, np), trn = planes(np, mp);
   Planes x = tall ? trn : nat, xt = tall ? nat : trn;
-  Planes xt2 = tall ? planes(mp, np) : planes(np, mp);
-  Planes g = planes(sp, sp), q = planes(sp, sp);
   const int parts = (int)std::min<int64_t>(
       std::max<int64_t>(1, 1024 / c.batch), (c.m * c.n + 4095) / 4096);
   auto part = at::empty({c.batch * parts}, c.options.dtype(at::kDouble));
@@ -1508,7 +1558,7 @@ void run_wide(const Chain& c) {
   for (const Cut& cut : {gram, poly, full})
     shared = std::max(shared, (cut.all - cut.whole) * cut.splits * cut.tile *
                                   cut.tile);
-  auto sums = at::empty({shared}, c.options.dtype(at::kFloat));
+  auto sums = at::empty({2 * shared}, c.options.dtype(at::kFloat));
   Product pr{};
   pr.ca = (float)c.k.a;
   pr.cb = (float)c.k.b;
@@ -1520,28 +1570,76 @@ void run_wide(const Chain& c) {
   pr.res = c.res;
   pr.parts = sums.data_ptr<float>();
   const int ks = round_up(s, 32), kl = round_up(long_, 32);
-  for (int i = 0; i < c.steps; ++i) {
-    pr.a = pr.b = x;
+  const float down = 1.0f / UP;
+  auto square = [&] { return planes(sp, sp); };
+  auto again = [&] { return tall ? planes(mp, np) : planes(np, mp); };
+  Planes g = square(), q = square(), xt2{};
+
+  auto new_gram = [&] {
+    pr.f[0] = {x, x, g, down};
     pr.k = kl;
-    pr.d = g;
     run_product<GRAM, T>(c, pr, gram);
-    pr.a = pr.b = g;
     pr.k = ks;
-    pr.d = q;
+  };
+  auto new_poly = [&](Planes to) {
+    pr.f[0] = {g, g, to, down};
     run_product<POLY, T>(c, pr, poly);
-    pr.a = q;
-    pr.b = xt;
-    pr.d = x;
+  };
+  // X <- (by / held) X, the last time as the result
+  auto apply = [&](Planes by, float held, bool last) {
+    if (last) {
+      pr.f[0] = {by, xt, x, down * down / held};
+      run_product<FINAL, T>(c, pr, full);
+      return;
+    }
+    if (!xt2.p) xt2 = again();
+    pr.f[0] = {by, xt, x, down / held};
     pr.dt = xt2;
-    if (i + 1 < c.steps) run_product<UPDATE, T>(c, pr, full);
-    else run_product<FINAL, T>(c, pr, full);
+    run_product<UPDATE, T>(c, pr, full);
     std::swap(xt, xt2);
+  };
+
+  new_gram();
+  if (!by_gram<T>(c, s, long_)) {
+    for (int i = 0; i < c.steps; ++i) {
+      if (i) new_gram();
+      new_poly(q);
+      apply(q, 1.0f, i + 1 == c.steps);
+    }
+    return;
   }
+  // Q from G; P <- P Q (the first P is Q); G <- Q (G Q)
+  Planes p = square(), p2 = square(), t = square(), g2 = square();
+  Reach reach;
+  float held = 1.0f;  // P's planes hold P times this
+  for (int i = 0; i < c.steps; ++i) {
+    const bool last = i + 1 == c.steps;
+    const Planes qi = i ? q : p;
+    new_poly(qi);
+    reach.step(c.k);
+    if (i) {
+      const float to = reach.hold();
+      pr.f[0] = {p, q, p2, down * (to / held)};
+      held = to;
+      pr.f[1] = {g, q, t, down};
+      run_product<GRAM, T>(c, pr, poly, last ? 1 : 2);
+      std::swap(p, p2);
+    } else {
+      pr.f[0] = {g, qi, t, down};
+      run_product<GRAM, T>(c, pr, poly);
+    }
+    if (!last) {
+      pr.f[0] = {qi, t, g2, down};
+      run_product<GRAM, T>(c, pr, poly);
+      std::swap(g, g2);
+    }
+  }
+  apply(p, held, true);
 }
 
 template <typename T>
 void run(const Chain& c) {
-  if (is_thin(c.m, c.n)) {
+  if (is_thin(c.batch, c.m, c.n)) {
     if (c.m >= c.n) run_thin<T, true>(c); else run_thin<T, false>(c);
   } else {
     run_wide<T>(c);
@@ -1560,7 +1658,7 @@ void dispatch(const Chain& whole) {
     at::Tensor active;
     if (c.touched) {
       c.touched += b;
-      if (!is_thin(c.m, c.n)) {
+      if (!is_thin(c.batch, c.m, c.n)) {
         active = at::empty({c.batch + 1}, c.options.dtype(at::kInt));
         c.active = active.data_ptr<int>();
         hipLaunchKernelGGL(k_active, dim3(1), dim3(1024), 0, c.stream,
@@ -1645,7 +1743,7 @@ void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
                    n,                         (float)mu,
                    nesterov};
   // one pass makes U and sums G where a block holds a row and a square of G
-  const bool fused = is_thin(matrix_rows, dim) && dim > NARROW &&
+  const bool fused = is_thin(batch, matrix_rows, dim) && dim > NARROW &&
                      dim <= SUPER && matrix_rows >= dim && batch <= 32768;
   if (!fused) {
     int group = 1;

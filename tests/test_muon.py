@@ -73,7 +73,8 @@ def matrices(kind, b, m, n, seed):
 SIZES = [(1, 1, 1), (1, 1, 50), (1, 50, 1), (4, 3, 5), (2, 16, 16),
          (3, 17, 33), (2, 64, 63), (1, 2000, 7), (1, 7, 2000), (1, 2500, 48),
          (1, 65, 65), (2, 100, 130), (2, 130, 100), (2, 200, 129),
-         (1, 257, 300), (1, 4200, 130), (1, 130, 4200)]
+         (1, 257, 300), (1, 4200, 130), (1, 130, 4200), (2, 128, 520),
+         (2, 520, 128), (5, 128, 520)]
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -107,6 +108,29 @@ def test_16_bit_types(device, dtype, m, n):
     got = ops.orthogonalize(x.to(device))
     for k in range(2):
         check(got[k], x[k])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", ["normal", "decay"])
+@pytest.mark.parametrize("steps,coeffs", [(1, ops.MUON_COEFFS),
+                                          (2, ops.MUON_COEFFS),
+                                          (5, ops.MUON_COEFFS),
+                                          (8, ops.MUON_COEFFS),
+                                          (11, ops.MUON_COEFFS),
+                                          (3, (1.5, -0.5, 0.0)),
+                                          (9, (1.875, -1.25, 0.375))])
+@pytest.mark.parametrize("m,n", [(140, 300), (300, 140), (130, 2100),
+                                 (520, 790)])
+def test_long_bfloat16_matrices(device, kind, steps, coeffs, m, n):
+    """The steps may be taken on the Gram matrix where that stays below
+    bfloat16's rounding: the error of the result is at most half as much
+    again as that of the exact result's rounding."""
+    x = matrices(kind, 2, m, n, 12).bfloat16()
+    got = ops.orthogonalize(x.to(device), steps=steps, coeffs=coeffs).cpu()
+    for k in range(2):
+        want, _ = chain(x[k], steps=steps, coeffs=coeffs)
+        rounding = float((want.bfloat16().double() - want).norm())
+        assert float((got[k].double() - want).norm()) <= 1.5 * rounding
 
 
 @pytest.mark.parametrize("device", DEVICES)
