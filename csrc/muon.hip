@@ -241,9 +241,8 @@ constexpr int SUPER = 128;     // a block's square of G
 constexpr int KC = 32;         // long-axis places a block stages at a time
 constexpr int PITCH = SUPER + 16;
 
-// What the chain leaves for the product that applies it: X = ((u x) y), and P
-// stands in its planes as P / z.
-struct Norm { float x, y, z; };
+// X = ((u x) y), what the product that applies P needs of the norm.
+struct Norm { float x, y; };
 
 // X = U / n with n = |U|_F + eps as (u x) y: the power of two x keeps y and
 // the products normal for values near the ends of f32's range.  NaN for a
@@ -272,17 +271,38 @@ __device__ inline double block_sum(double v, double* lds) {
   return v;
 }
 
+// NT neighbours, those before `held` (any number), zeros after them
+template <int NT, typename T>
+__device__ inline void load_some(float (&v)[NT], const T* at, int64_t held) {
+  if (NT == 4) {
+    const float4 f = load_quad(at, held);
+    v[0] = f.x;
+    v[1 % NT] = f.y;
+    v[2 % NT] = f.z;
+    v[3 % NT] = f.w;
+  } else if (NT == 2 && held >= 2) {
+    Pair<T> p;
+    p.load(at);
+    v[0] = to_f32(p.get(0));
+    v[1 % NT] = to_f32(p.get(1));
+  } else {
+    v[0] = held > 0 ? to_f32(at[0]) : 0.0f;
+    if (NT == 2) v[1 % NT] = 0.0f;
+  }
+}
+
 // Partial sums of G over one chunk of the long axis, short side up to
-// 16 NT <= 64: part[b][chunk][sp][sp], tiles on and under the diagonal.
-// f64 matrix instructions 16x16x4: a lane holds row (or column) lane % 16 at
-// place lane / 16; the order of the places is free, so four neighbouring ones
-// serve four instructions.  No LDS on the way: a wave reads its own places,
-// and four waves' sums are joined at the end.
+// 16 NT <= 64.  f64 matrix instructions 16x16x4: a lane holds row (or column)
+// lane % 16 of a tile at place lane / 16.  Both orders are free: tile t takes
+// columns NT c + t, so that a lane's values lie side by side, and four
+// neighbouring places serve four instructions.  No LDS on the way: a wave reads
+// its own places, the next ones while it multiplies, and four waves' sums are
+// joined at the end.  part[b][chunk][tile (i, j <= i)][16][16].
 template <typename T, bool TALL, int NT>
 __global__ __launch_bounds__(256) void k_gram_narrow(
     double* __restrict__ part, const T* __restrict__ u,
     const int* __restrict__ touched, int64_t long_, int s, int64_t chunk) {
-  constexpr int SP = NT * 16, TILES = NT * (NT + 1) / 2;
+  constexpr int TILES = NT * (NT + 1) / 2;
   __shared__ double lds[TILES * 256];
   const int64_t b = blockIdx.y;
   if (touched && !touched[b]) return;
@@ -294,20 +314,21 @@ __global__ __launch_bounds__(256) void k_gram_narrow(
 #pragma unroll
   for (int t = 0; t < TILES; ++t) acc[t] = (f64x4){0, 0, 0, 0};
   constexpr int TURNS = NT > 2 ? 1 : 2;  // 16 places each, loaded together
-  for (int64_t k = k0; k < k1; k += 16 * TURNS) {
-    float v[TURNS][4][NT];
+  float v[TURNS][4][NT];
+  auto fetch = [&](int64_t k) {
 #pragma unroll
-    for (int h = 0; h < TURNS; ++h)
+    for (int h = 0; h < TURNS; ++h) {
+      if (TALL) {
+        const int col = lane % 16 * NT;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int col = t * 16 + lane % 16;
-        if (TALL) {
+        for (int c = 0; c < 4; ++c) {
+          const int64_t kk = k + h * 16 + 4 * c + lane / 16;
+          load_some<NT>(v[h][c], x + kk * s + col, kk < k1 ? s - col : 0);
+        }
+      } else {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int64_t kk = k + h * 16 + 4 * c + lane / 16;
-            v[h][c][t] = col < s && kk < k1 ? to_f32(x[kk * s + col]) : 0.0f;
-          }
-        } else {
+        for (int t = 0; t < NT; ++t) {
+          const int col = lane % 16 * NT + t;
           const int64_t kk = k + h * 16 + lane / 16 * 4;
           const float4 f = load_quad(x + col * long_ + kk,
                                      col < s ? k1 - kk : 0);
@@ -317,6 +338,18 @@ __global__ __launch_bounds__(256) void k_gram_narrow(
           v[h][3][t] = f.w;
         }
       }
+    }
+  };
+  fetch(k0);
+  for (int64_t k = k0; k < k1; k += 16 * TURNS) {
+    double w[TURNS][4][NT];
+#pragma unroll
+    for (int h = 0; h < TURNS; ++h)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) w[h][c][t] = v[h][c][t];
+    fetch(k + 16 * TURNS);
 #pragma unroll
     for (int h = 0; h < TURNS; ++h)
 #pragma unroll
@@ -326,7 +359,7 @@ __global__ __launch_bounds__(256) void k_gram_narrow(
 #pragma unroll
           for (int j = 0; j <= i; ++j)
             acc[i * (i + 1) / 2 + j] = __builtin_amdgcn_mfma_f64_16x16x4f64(
-                v[h][c][i], v[h][c][j], acc[i * (i + 1) / 2 + j], 0, 0, 0);
+                w[h][c][i], w[h][c][j], acc[i * (i + 1) / 2 + j], 0, 0, 0);
   }
   for (int w = 0; w < 4; ++w) {
     if (wave == w) {
@@ -340,13 +373,34 @@ __global__ __launch_bounds__(256) void k_gram_narrow(
     }
     __syncthreads();
   }
-  double* out = part + (b * gridDim.x + blockIdx.x) * (int64_t)SP * SP;
-  int ti = 0, tj = 0;
-  for (int t = 0; t < TILES; ++t) {
-    out[(ti * 16 + threadIdx.x / 16) * SP + tj * 16 + threadIdx.x % 16] =
-        lds[t * 256 + threadIdx.x];
-    if (++tj > ti) { tj = 0; ++ti; }
-  }
+  double* out = part + (b * gridDim.x + blockIdx.x) * (int64_t)(TILES * 256);
+#pragma unroll
+  for (int t = 0; t < TILES; ++t)
+    out[t * 256 + threadIdx.x] = lds[t * 256 + threadIdx.x];
+}
+
+// sum[b][size] = the chunks' sum, in an order of its own that does not change:
+// 16 values a block, 16 threads a value.
+__global__ __launch_bounds__(256) void k_part_sum(
+    double* __restrict__ sum, const double* __restrict__ part,
+    const int* __restrict__ touched, int chunks, int64_t size) {
+  __shared__ double slices[16][17];
+  const int64_t b = blockIdx.y;
+  if (touched && !touched[b]) return;
+  const int64_t e = (int64_t)blockIdx.x * 16 + threadIdx.x % 16;
+  const double* p = part + b * chunks * size + e;
+  double v[4] = {0, 0, 0, 0};
+  int k = threadIdx.x / 16;
+  for (; k + 48 < chunks; k += 64)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] += p[(k + q * 16) * size];
+  for (; k < chunks; k += 16) v[0] += p[k * size];
+  slices[threadIdx.x / 16][threadIdx.x % 16] = (v[0] + v[1]) + (v[2] + v[3]);
+  __syncthreads();
+  if (threadIdx.x >= 16) return;
+  double t = 0;
+  for (int q = 0; q < 16; ++q) t += slices[q][threadIdx.x];
+  sum[b * size + e] = t;
 }
 
 // KC places of a diagonal square of G, 8 x 8 tiles of which nt x nt exist:
@@ -394,35 +448,42 @@ __device__ inline void diagonal_tiles(const f64x4 (&acc)[N], F f) {
   }
 
 // The same for short sides up to THIN_MAX: a block takes the places of one
-// chunk for a SUPER x SUPER square of G, through LDS (two buffers, one barrier
-// a turn).  The matrix instructions bound it: 64 cycles a tile and 4 places.
+// chunk for a SUPER x SUPER square of G on the diagonal, or for half of one under
+// it, through LDS (two buffers, one barrier a turn), nine or eight tiles a wave.
+// The matrix instructions bound it: 64 cycles a tile and 4 places.
+// part[b][chunk][sp][sp].
 //
 // With STEP (tall, one square) the values are those of U as the momentum
 // makes it: M and the gradients come in, M and U go out on the way.
 template <typename T, bool TALL, bool STEP>
-__global__ __launch_bounds__(256, STEP ? 2 : 1) void k_gram64(
+__global__ __launch_bounds__(256, 2) void k_gram64(
     double* __restrict__ part, double* __restrict__ traces,
     const T* __restrict__ u, Momentum mom, const int64_t* __restrict__ place,
     const int* __restrict__ touched, int64_t long_, int s, int sp,
     int64_t chunk) {
-  __shared__ float lds[STEP ? 2 : 4][KC][PITCH];
+  constexpr int HALF = SUPER / 2, HPITCH = HALF + 16;
+  __shared__ float lds[2][KC][PITCH];
+  __shared__ float other[STEP ? 1 : 2][KC][HPITCH];  // the half's rows
   __shared__ double sums[4];
   const int64_t b = blockIdx.z;
   if (touched && !touched[b]) return;
-  // blockIdx.y counts the pairs of super-tiles (si >= sj)
-  int si = 0, sj = STEP ? 0 : blockIdx.y;
-  while (sj > si) { sj -= si + 1; ++si; }
+  // blockIdx.y: of each row of squares first the halves, then the diagonal one
+  int si = 0, y = STEP ? 0 : blockIdx.y;
+  while (y > 2 * si) { y -= 2 * si + 1; ++si; }
+  const int sj = y / 2;
   const bool diagonal = STEP || si == sj;
-  const int ni = min(8, sp / 16 - si * 8), nj = min(8, sp / 16 - sj * 8);
+  const int row0 = si * SUPER + (diagonal ? 0 : y % 2 * HALF);
+  const int col0 = sj * SUPER;
+  const int nt = min(8, (sp - col0) / 16);  // tiles of its columns
+  if (row0 >= sp) return;                   // no such half
   const int lane = threadIdx.x % WAVE, wave = this_wave();
   const T* x = u + b * long_ * s;
   const int64_t k0 = blockIdx.x * chunk;
   const int64_t k1 = min(k0 + chunk, long_);
 
-  constexpr int TILES = STEP ? 9 : 16;  // a wave's, at most
-  f64x4 acc[TILES];
+  f64x4 acc[9];
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) acc[t] = (f64x4){0, 0, 0, 0};
+  for (int t = 0; t < 9; ++t) acc[t] = (f64x4){0, 0, 0, 0};
 
   // STEP: the places are known a turn ahead of the values
   int64_t at_[4];
@@ -434,8 +495,15 @@ __global__ __launch_bounds__(256, STEP ? 2 : 1) void k_gram64(
     }
   };
 
-  // four quads a thread: along the columns (TALL) or along the places
-  float4 next[2][4];
+  // Quads along the columns (TALL) or along the places: four of the square's
+  // columns a thread, and two of the half's rows (STEP: four gradients).
+  float4 next[4], more[STEP ? 4 : 2];
+  auto some = [&](int64_t k, int kk, int col) {
+    return load_quad(TALL ? x + (k + kk) * s + col
+                          : x + (int64_t)col * long_ + k + kk,
+                     TALL ? (k + kk < k1 ? (int64_t)s - col : 0)
+                          : (col < s ? k1 - k - kk : 0));
+  };
   auto fetch = [&](int64_t k) {
 #pragma unroll
     for (int l = 0; l < 4; ++l) {
@@ -444,20 +512,29 @@ __global__ __launch_bounds__(256, STEP ? 2 : 1) void k_gram64(
       if (STEP) {
         const int held = k + kk < k1 ? s - c : 0;
         const int64_t row = b * long_ + k + kk;
-        next[0][l] = load_quad(mom.m + row * s + c, held);
-        next[1][l] = row_gradient(mom, at_[l], row, s, c, held);
-        continue;
+        next[l] = load_quad(mom.m + row * s + c, held);
+        more[l % (STEP ? 4 : 2)] = row_gradient(mom, at_[l], row, s, c, held);
+      } else {
+        next[l] = some(k, kk, col0 + c);
       }
+    }
+    if (!STEP && !diagonal) {
 #pragma unroll
-      for (int o = 0; o < 2; ++o) {
-        if (o && diagonal) continue;
-        const int col = (o ? sj : si) * SUPER + c;
-        const int64_t held = TALL ? (k + kk < k1 ? s - col : 0)
-                                  : (col < s ? k1 - k - kk : 0);
-        next[o][l] = load_quad(TALL ? x + (k + kk) * s + col
-                                    : x + (int64_t)col * long_ + k + kk,
-                               held);
+      for (int l = 0; l < 2; ++l) {
+        const int e = threadIdx.x + l * 256;
+        more[l] = some(k, TALL ? e / 16 : e % 8 * 4,
+                       row0 + (TALL ? e % 16 * 4 : e / 8));
       }
+    }
+  };
+  auto put_some = [&](float* to, int pitch, float4 f) {
+    if (TALL) {
+      *(float4*)to = f;
+    } else {
+      to[0] = f.x;
+      to[pitch] = f.y;
+      to[2 * pitch] = f.z;
+      to[3 * pitch] = f.w;
     }
   };
   auto put = [&](int64_t k, int buffer) {
@@ -465,29 +542,24 @@ __global__ __launch_bounds__(256, STEP ? 2 : 1) void k_gram64(
     for (int l = 0; l < 4; ++l) {
       const int e = threadIdx.x + l * 256;
       const int kk = TALL ? e / 32 : e % 8 * 4, c = TALL ? e % 32 * 4 : e / 8;
+      float4 v = next[l];
       if (STEP) {
         const int held = k + kk < k1 ? s - c : 0;
         const int64_t at = (b * long_ + k + kk) * s + c;
-        float4 v;
-        const float4 m = next_momentum(mom, next[0][l], next[1][l], &v);
+        const float4 m = next_momentum(mom, next[l],
+                                       more[l % (STEP ? 4 : 2)], &v);
         store_quad(mom.m + at, m, held);
         store_quad(mom.u + at, v, held);
-        *(float4*)&lds[buffer][kk][c] = v;
-        continue;
       }
+      put_some(&lds[buffer][kk][c], PITCH, v);
+    }
+    if (!STEP && !diagonal) {
 #pragma unroll
-      for (int o = 0; o < 2; ++o) {
-        if (o && diagonal) continue;
-        float (*to)[PITCH] = lds[buffer + (STEP ? 0 : o * 2)];
-        const float4 f = next[o][l];
-        if (TALL) {
-          *(float4*)&to[kk][c] = f;
-        } else {
-          to[kk][c] = f.x;
-          to[kk + 1][c] = f.y;
-          to[kk + 2][c] = f.z;
-          to[kk + 3][c] = f.w;
-        }
+      for (int l = 0; l < 2; ++l) {
+        const int e = threadIdx.x + l * 256;
+        put_some(&other[STEP ? 0 : buffer][TALL ? e / 16 : e % 8 * 4]
+                       [TALL ? e % 16 * 4 : e / 8],
+                 HPITCH, more[l]);
       }
     }
   };
@@ -499,46 +571,40 @@ __global__ __launch_bounds__(256, STEP ? 2 : 1) void k_gram64(
   int buffer = 0;
   for (int64_t k = k0; k < k1; k += KC) {
     __syncthreads();
-    const bool more = k + KC < k1;
-    if (more) {
+    const bool again = k + KC < k1;
+    if (again) {
       fetch(k + KC);
       look(k + 2 * KC);
     }
-    const float (*rows)[PITCH] = lds[buffer];
+    const float (*cols)[PITCH] = lds[buffer];
     if (diagonal) {
-      BY_WAVE(wave, diagonal_places<W>(acc, rows, lane, ni))
-    } else if constexpr (!STEP) {
-      const float (*cols)[PITCH] = lds[buffer + 2];
+      BY_WAVE(wave, diagonal_places<W>(acc, cols, lane, nt))
+    } else if (row0 + wave * 16 < sp) {
+      const float (*rows)[HPITCH] = other[STEP ? 0 : buffer];
 #pragma unroll
       for (int q = 0; q < KC; q += 4) {
         const int kk = q + lane / 16;
-        double av[2], bv[8];
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-          av[p] = rows[kk][(wave + p * 4) * 16 + lane % 16];
+        const double av = rows[kk][wave * 16 + lane % 16];
+        double bv[8];
 #pragma unroll
         for (int t = 0; t < 8; ++t) bv[t] = cols[kk][t * 16 + lane % 16];
 #pragma unroll
-        for (int p = 0; p < 2; ++p)
-          if (wave + p * 4 < ni) {
-#pragma unroll
-            for (int t = 0; t < 8; ++t)
-              acc[p * 8 + t] = __builtin_amdgcn_mfma_f64_16x16x4f64(
-                  av[p], bv[t], acc[p * 8 + t], 0, 0, 0);
-          }
+        for (int t = 0; t < 8; ++t)  // all of them exist left of the diagonal
+          acc[t] = __builtin_amdgcn_mfma_f64_16x16x4f64(av, bv[t], acc[t], 0,
+                                                        0, 0);
       }
     }
-    if (more) put(k + KC, buffer ^ 1);
+    if (again) put(k + KC, buffer ^ 1);
     buffer ^= 1;
   }
   double* out = part + (b * gridDim.x + blockIdx.x) * (int64_t)sp * sp;
   double trace = 0;
   auto keep = [&](int ti, int tj, const f64x4& v) {
-    if (ti >= ni || tj >= nj) return;
+    const int i0 = row0 + ti * 16, j0 = col0 + tj * 16;
+    if (i0 >= sp || j0 >= sp) return;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = si * SUPER + ti * 16 + lane / 16 + 4 * r;
-      const int j = sj * SUPER + tj * 16 + lane % 16;
+      const int i = i0 + lane / 16 + 4 * r, j = j0 + lane % 16;
       out[(int64_t)i * sp + j] = v[r];
       if (i == j) trace += v[r];
     }
@@ -549,11 +615,9 @@ __global__ __launch_bounds__(256, STEP ? 2 : 1) void k_gram64(
     if (threadIdx.x == 0)
       traces[(b * gridDim.x + blockIdx.x) * ((sp + SUPER - 1) / SUPER) + si] =
           trace;
-  } else if constexpr (!STEP) {
+  } else {
 #pragma unroll
-    for (int p = 0; p < 2; ++p)
-#pragma unroll
-      for (int t = 0; t < 8; ++t) keep(wave + p * 4, t, acc[p * 8 + t]);
+    for (int t = 0; t < 8; ++t) keep(wave, t, acc[t]);
   }
 }
 
@@ -572,7 +636,7 @@ __global__ __launch_bounds__(256) void k_gram_sum(
   const double2 f = norm_factors(block_sum(t, sums), eps);
   const double nu = f.x * f.y;
   if (blockIdx.x == 0 && threadIdx.x == 0)
-    norm[b] = Norm{(float)f.x, (float)f.y, 0.0f};
+    norm[b] = Norm{(float)f.x, (float)f.y};
   // 16 values a block, 16 threads a value
   __shared__ double slices[16][17];
   const int64_t size = (int64_t)sp * sp;
@@ -643,42 +707,20 @@ __global__ __launch_bounds__(256) void k_small_mul(
   job.out[ta] = v;
 }
 
-// P into two f16 planes of jp x kp places (zeros around it), scaled by a power
-// of two that takes its largest value to 2^12.  The block's threads together;
-// p(i, j) reads P.
-template <typename P>
-__device__ inline void put_planes(_Float16* planes, int64_t plane, int jp,
-                                  int kp, int s, P p, Norm* norm,
-                                  double* lds) {
-  double top = 0;
-  for (int e = threadIdx.x; e < s * s; e += blockDim.x)
-    top = fmax(top, fabs(p(e / s, e % s)));
-#pragma unroll
-  for (int o = WAVE / 2; o; o >>= 1) top = fmax(top, __shfl_xor(top, o));
-  __syncthreads();
-  if (threadIdx.x % WAVE == 0) lds[threadIdx.x / WAVE] = top;
-  __syncthreads();
-  for (int w = 0; w < (int)blockDim.x / WAVE; ++w) top = fmax(top, lds[w]);
-  const int e2 = top > 0 && top < INFINITY ? 12 - ilogb(top) : 0;
-  for (int e = threadIdx.x; e < jp * kp; e += blockDim.x) {
-    const int i = e / kp, j = e % kp;
-    const float v = i < s && j < s ? (float)ldexp(p(i, j), e2) : 0.0f;
-    split(v, planes[e], planes[plane + e]);
-  }
-  if (threadIdx.x == 0) norm->z = (float)ldexp(1.0, -e2);
-}
-
-__global__ __launch_bounds__(1024) void k_small_out(
+// `by` P in two f16 planes of jp x kp places, zeros around it
+__global__ __launch_bounds__(256) void k_small_out(
     _Float16* __restrict__ planes, const double* __restrict__ p,
-    Norm* __restrict__ norm, const int* __restrict__ touched, int s, int sp,
-    int jp, int kp) {
-  __shared__ double lds[16];
-  const int64_t b = blockIdx.x;
+    const int* __restrict__ touched, int s, int sp, int jp, int kp,
+    double by) {
+  const int64_t b = blockIdx.y;
   if (touched && !touched[b]) return;
-  const double* at = p + b * (int64_t)sp * sp;
-  put_planes(planes + b * (int64_t)jp * kp, gridDim.x * (int64_t)jp * kp, jp,
-             kp, s, [&](int i, int j) { return at[i * sp + j]; }, norm + b,
-             lds);
+  const int e = blockIdx.x * 256 + threadIdx.x;
+  if (e >= jp * kp) return;
+  const int i = e / kp, j = e % kp;
+  const int64_t plane = gridDim.y * (int64_t)jp * kp;
+  _Float16* to = planes + b * (int64_t)jp * kp + e;
+  split(i < s && j < s ? (float)(p[(b * sp + i) * sp + j] * by) : 0.0f, to[0],
+        to[plane]);
 }
 
 // The chain for short sides up to 64: one block a matrix, G, Q, P and G Q in
@@ -688,7 +730,8 @@ template <int NT, int WAVES>
 __global__ __launch_bounds__(WAVES * WAVE) void k_chain(
     _Float16* __restrict__ planes, Norm* __restrict__ norm,
     const double* __restrict__ part, const int* __restrict__ touched,
-    int chunks, int s, int steps, Coeffs k, double eps, int jp, int kp) {
+    int chunks, int s, int steps, Coeffs k, double eps, int jp, int kp,
+    double by) {
   constexpr int SP = NT * 16, LP = SP + 2, TILES = NT * (NT + 1) / 2;
   // tiles of two products at a time
   constexpr int MINE = (2 * TILES + WAVES - 1) / WAVES;
@@ -697,34 +740,28 @@ __global__ __launch_bounds__(WAVES * WAVE) void k_chain(
   const int64_t b = blockIdx.x;
   if (touched && !touched[b]) return;
   const int lane = threadIdx.x % WAVE, wave = this_wave();
-  const double* from = part + b * chunks * (int64_t)SP * SP;
+  const double* from = part + b * chunks * (int64_t)(TILES * 256);
 
   // the sum of the parts: 256 threads take a value of every tile each, and
   // every (WAVES / 4)-th part
   const int slice = wave / 4, e = threadIdx.x % 256;
   double sum[TILES] = {};
-#pragma unroll 4
-  for (int c = slice; c < chunks; c += WAVES / 4) {
-    int ti = 0, tj = 0;
+#pragma unroll 8
+  for (int c = slice; c < chunks; c += WAVES / 4)
 #pragma unroll
-    for (int o = 0; o < TILES; ++o) {
-      sum[o] += from[((int64_t)c * SP + ti * 16 + e / 16) * SP + tj * 16 +
-                     e % 16];
-      if (++tj > ti) { tj = 0; ++ti; }
-    }
-  }
+    for (int o = 0; o < TILES; ++o)
+      sum[o] += from[((int64_t)c * TILES + o) * 256 + e];
   for (int w = 0; w < WAVES / 4; ++w) {
     if (slice == w) {
       int ti = 0, tj = 0;
 #pragma unroll
       for (int o = 0; o < TILES; ++o) {
-        const int i = ti * 16 + e / 16, j = tj * 16 + e % 16;
-        if (i >= j) {
-          double v = sum[o];
-          if (w) v += g[i * LP + j];
-          g[i * LP + j] = v;
-          g[j * LP + i] = v;
-        }
+        // as k_gram_narrow orders them
+        const int i = e / 16 * NT + ti, j = e % 16 * NT + tj;
+        double v = sum[o];
+        if (w) v += g[i * LP + j];
+        g[i * LP + j] = v;
+        if (ti != tj) g[j * LP + i] = v;
         if (++tj > ti) { tj = 0; ++ti; }
       }
     }
@@ -733,7 +770,7 @@ __global__ __launch_bounds__(WAVES * WAVE) void k_chain(
   const double trace = threadIdx.x < SP ? g[threadIdx.x * (LP + 1)] : 0.0;
   const double2 f = norm_factors(block_sum(trace, sums), eps);
   const double nu = f.x * f.y;
-  if (threadIdx.x == 0) norm[b] = Norm{(float)f.x, (float)f.y, 0.0f};
+  if (threadIdx.x == 0) norm[b] = Norm{(float)f.x, (float)f.y};
   for (int o = threadIdx.x; o < SP * LP; o += WAVES * WAVE)
     if (o % LP < SP) g[o] *= nu * nu;
   __syncthreads();
@@ -798,89 +835,93 @@ __global__ __launch_bounds__(WAVES * WAVE) void k_chain(
     else if (!last) mul(grow, none, false);
     if (!last) mul({g, qi, t}, none, false);
   }
-  put_planes(planes + b * (int64_t)jp * kp, gridDim.x * (int64_t)jp * kp, jp,
-             kp, s, [&](int i, int j) { return p[i * LP + j]; }, norm + b,
-             sums);
+  const int64_t plane = gridDim.x * (int64_t)jp * kp;
+  for (int o = threadIdx.x; o < jp * kp; o += WAVES * WAVE) {
+    const int i = o / kp, j = o % kp;
+    _Float16* to = planes + b * (int64_t)jp * kp + o;
+    split(i < s && j < s ? (float)(p[i * LP + j] * by) : 0.0f, to[0],
+          to[plane]);
+  }
 }
 
-// O = U P (TALL) or P U: P in LDS, 16 JT places of the short side and KS
-// places of the sum at a time; a wave 32 places of the long axis a turn, whose
-// values it takes from memory to the matrix instructions by itself, split in
-// two planes on the way.  Bound by memory.
-template <typename T, bool TALL, int JT, int KS>
-__global__ __launch_bounds__(256) void k_thin_apply(
+// O = U P (TALL) or P U: 16 JT of P's rows, up to KS places long, in LDS; a wave
+// takes its values from memory to the matrix instructions by itself, split in
+// two planes on the way, CH places of the sum at a time.  A lane holds eight
+// places of long-axis row lane % 16 (TALL: its neighbours in memory), or of
+// four neighbouring ones, which lie in four tiles.  Bound by memory.
+template <typename T, bool TALL, int JT, int KS, int WAVES>
+__global__ __launch_bounds__(WAVES * WAVE) void k_thin_apply(
     Result res, const T* __restrict__ u, const _Float16* __restrict__ planes,
     const Norm* __restrict__ norm, const int* __restrict__ touched,
-    int64_t long_, int s, int jp, int kp) {
+    int64_t long_, int s, int jp, int kp, float down) {
   constexpr int LP = KS + 8;  // rows of eight lanes' pieces in other banks
+  constexpr int RT = TALL ? 2 : 4;         // tiles of the long axis a wave
+  constexpr int TURN = WAVES * 16 * RT;    // places of it a block and turn
+  constexpr int CH = KS < 64 ? 32 : TALL && KS == 128 ? 128 : 64;
   __shared__ _Float16 lds[2][JT * 16 * LP];
   const int64_t b = blockIdx.z;
   if (touched && !touched[b]) return;
   const int lane = threadIdx.x % WAVE, wave = this_wave();
   const int j0 = blockIdx.y * JT * 16;
   const Norm nm = norm[b];
-  const float up = nm.y * UP, down = nm.z / UP;
+  const float up = nm.y * UP;
   const T* x = u + b * long_ * s;
   const _Float16* p = planes + (b * jp + j0) * (int64_t)kp;
   const int64_t plane = gridDim.z * (int64_t)jp * kp;
-  const int kchunks = (kp + KS - 1) / KS;
+  for (int e = threadIdx.x; e < 2 * JT * 16 * (KS / 8); e += WAVES * WAVE) {
+    const int h = e / (JT * 16 * (KS / 8)), r = e / (KS / 8) % (JT * 16);
+    const int c = e % (KS / 8) * 8;
+    half8 v = {};
+    if (c < kp) v = *(const half8*)(p + h * plane + (int64_t)r * kp + c);
+    *(half8*)&lds[h][r * LP + c] = v;
+  }
+  __syncthreads();
 
-  auto stage = [&](int kc) {
-    __syncthreads();
-    for (int e = threadIdx.x; e < 2 * JT * 16 * (KS / 8); e += 256) {
-      const int h = e / (JT * 16 * (KS / 8)), r = e / (KS / 8) % (JT * 16);
-      const int c = e % (KS / 8) * 8;
-      half8 v = {};
-      if (kc + c < kp)
-        v = *(const half8*)(p + h * plane + (int64_t)r * kp + kc + c);
-      *(half8*)&lds[h][r * LP + c] = v;
-    }
-    __syncthreads();
-  };
-  if (kchunks == 1) stage(0);
-
-  for (int64_t base = (int64_t)blockIdx.x * 128; base < long_;
-       base += (int64_t)gridDim.x * 128) {
-    f32x4 acc[JT][2];
+  for (int64_t base = (int64_t)blockIdx.x * TURN + wave * (16 * RT);
+       base < long_; base += (int64_t)gridDim.x * TURN) {
+    // the long-axis place of the lane's row in tile w
+    const int64_t r0 = base + (TALL ? lane % 16 : lane % 16 * 4);
+    auto at = [&](int w) { return r0 + w * (TALL ? 16 : 1); };
+    f32x4 acc[JT][RT];
 #pragma unroll
     for (int t = 0; t < JT; ++t)
 #pragma unroll
-      for (int w = 0; w < 2; ++w) acc[t][w] = (f32x4){0, 0, 0, 0};
-    const int64_t r0 = base + wave * 32 + lane % 16;
-    for (int kc = 0; kc < kp; kc += KS) {
-      if (kchunks > 1) stage(kc);
-      float raw[KS / 32][2][8];
+      for (int w = 0; w < RT; ++w) acc[t][w] = (f32x4){0, 0, 0, 0};
+    for (int kc = 0; kc < kp; kc += CH) {
+      float raw[CH / 32][RT][8];
 #pragma unroll
-      for (int ks = 0; ks < KS / 32; ++ks)
+      for (int ks = 0; ks < CH / 32; ++ks) {
+        const int k = kc + ks * 32 + lane / 16 * 8;
+        if (TALL) {
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int64_t r = r0 + w * 16;
-          const int k = kc + ks * 32 + lane / 16 * 8;
-          if (TALL) {
-            const int held = r < long_ ? s - k : 0;
-            const float4 f = load_quad(x + r * s + k, held);
-            const float4 g = load_quad(x + r * s + k + 4, held - 4);
-            raw[ks][w][0] = f.x;
-            raw[ks][w][1] = f.y;
-            raw[ks][w][2] = f.z;
-            raw[ks][w][3] = f.w;
-            raw[ks][w][4] = g.x;
-            raw[ks][w][5] = g.y;
-            raw[ks][w][6] = g.z;
-            raw[ks][w][7] = g.w;
-          } else {
+          for (int w = 0; w < RT; ++w)
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-              raw[ks][w][c] = r < long_ && k + c < s
-                                  ? to_f32(x[(int64_t)(k + c) * long_ + r])
-                                  : 0.0f;
+            for (int h = 0; h < 2; ++h) {
+              const float4 f = load_quad(x + at(w) * s + k + h * 4,
+                                         at(w) < long_ ? s - k - h * 4 : 0);
+              raw[ks][w][h * 4] = f.x;
+              raw[ks][w][h * 4 + 1] = f.y;
+              raw[ks][w][h * 4 + 2] = f.z;
+              raw[ks][w][h * 4 + 3] = f.w;
+            }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const float4 f = load_quad(x + (k + c) * long_ + r0,
+                                       k + c < s ? long_ - r0 : 0);
+            raw[ks][0][c] = f.x;
+            raw[ks][1][c] = f.y;
+            raw[ks][2 % RT][c] = f.z;
+            raw[ks][3 % RT][c] = f.w;
           }
         }
+      }
 #pragma unroll
-      for (int ks = 0; ks < KS / 32; ++ks) {
-        half8 hi[2], lo[2];
+      for (int ks = 0; ks < CH / 32; ++ks) {
+        if (KS > 128 && kc + ks * 32 >= kp) continue;
+        half8 hi[RT], lo[RT];
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
+        for (int w = 0; w < RT; ++w)
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             _Float16 h, l;
@@ -890,11 +931,12 @@ __global__ __launch_bounds__(256) void k_thin_apply(
           }
 #pragma unroll
         for (int t = 0; t < JT; ++t) {
-          const int at = (t * 16 + lane % 16) * LP + ks * 32 + lane / 16 * 8;
-          const half8 ph = *(const half8*)&lds[0][at];
-          const half8 pl = *(const half8*)&lds[1][at];
+          const int from = (t * 16 + lane % 16) * LP + kc + ks * 32 +
+                           lane / 16 * 8;
+          const half8 ph = *(const half8*)&lds[0][from];
+          const half8 pl = *(const half8*)&lds[1][from];
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
+          for (int w = 0; w < RT; ++w) {
             acc[t][w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                 pl, hi[w], acc[t][w], 0, 0, 0);
             acc[t][w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
@@ -905,25 +947,26 @@ __global__ __launch_bounds__(256) void k_thin_apply(
         }
       }
     }
+    const int64_t mine = b * long_ * s;
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const int64_t r = r0 + w * 16;
-      if (r >= long_) continue;
+    for (int t = 0; t < JT; ++t) {
+      const int j = j0 + t * 16 + lane / 16 * 4;
+      if (TALL) {
 #pragma unroll
-      for (int t = 0; t < JT; ++t) {
-        const int j = j0 + t * 16 + lane / 16 * 4;
-        const float4 o = make_float4(acc[t][w][0] * down, acc[t][w][1] * down,
-                                     acc[t][w][2] * down, acc[t][w][3] * down);
-        if (TALL) {
-          finish_quad<T>(res, b * long_ * s + r * s + j, o, s - j);
-        } else {
-          const float v[4] = {o.x, o.y, o.z, o.w};
+        for (int w = 0; w < RT; ++w)
+          finish_quad<T>(res, mine + at(w) * s + j,
+                         make_float4(acc[t][w][0] * down, acc[t][w][1] * down,
+                                     acc[t][w][2] * down,
+                                     acc[t][w][3] * down),
+                         at(w) < long_ ? s - j : 0);
+      } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (j + i < s)
-              finish<T>(res, b * long_ * s + (int64_t)(j + i) * long_ + r,
-                        v[i]);
-        }
+        for (int i = 0; i < 4; ++i)
+          finish_quad<T>(res, mine + (int64_t)(j + i) * long_ + r0,
+                         make_float4(acc[t][0][i] * down, acc[t][1][i] * down,
+                                     acc[t][2 % RT][i] * down,
+                                     acc[t][3 % RT][i] * down),
+                         j + i < s ? long_ - r0 : 0);
       }
     }
   }
@@ -1340,6 +1383,30 @@ bool is_thin(int64_t batch, int64_t m, int64_t n) {
 }
 
 
+// How far P's values can reach: its value at singular values from 0 to 1.
+struct Reach {
+  double x[257], p[257];
+  Reach() {
+    for (int i = 0; i < 257; ++i) {
+      x[i] = i / 256.0;
+      p[i] = 1.0;
+    }
+  }
+  void step(const Coeffs& k) {
+    for (int i = 0; i < 257; ++i) {
+      const double y = x[i] * x[i], q = k.a + k.b * y + k.c * y * y;
+      p[i] *= q;
+      x[i] *= q;
+    }
+  }
+  // the power of two that keeps P under 4, up to what lies between the points
+  float hold() const {
+    double top = 0;
+    for (double v : p) top = std::max(top, std::abs(v));
+    return top > 4 ? (float)std::exp2(-std::ceil(std::log2(top / 4))) : 1.0f;
+  }
+};
+
 template <typename T, bool TALL>
 void run_thin(const Chain& c) {
   const int s = std::min(c.m, c.n);
@@ -1347,44 +1414,60 @@ void run_thin(const Chain& c) {
   const bool narrow = s <= NARROW;
   const int nt = !narrow ? (s + 15) / 16 : s <= 16 ? 1 : s <= 32 ? 2 : 4;
   const int sp = nt * 16;
-  const int super = (s + SUPER - 1) / SUPER, pairs = super * (super + 1) / 2;
-  // chunks: about two blocks a CU, of at least 64 places (16 a wave) or KC
+  // blocks of G's squares: one on the diagonal, two under it
+  const int super = (s + SUPER - 1) / SUPER, squares = super * super;
+  // chunks: about two blocks a CU (four where a block needs little), of at
+  // least 64 places (16 a wave) or KC
   const int64_t least = narrow ? 64 : KC;
   int64_t chunks = std::min<int64_t>(
       (long_ + least - 1) / least,
-      std::max<int64_t>(1, 512 / (c.batch * (narrow ? 1 : pairs))));
+      std::max<int64_t>(1, narrow ? 1024 / c.batch
+                                  : 512 / (c.batch * squares)));
   const int64_t chunk = round_up((long_ + chunks - 1) / chunks, least);
   chunks = (long_ + chunk - 1) / chunk;
-  const int64_t size = (int64_t)sp * sp;
-  // the planes of P: JT * 16 rows a block, KS places of the sum
-  const int jt = s <= 32 ? 2 : s <= 64 ? 4 : 8;
+  const int64_t size = narrow ? nt * (nt + 1) / 2 * 256 : (int64_t)sp * sp;
+  // the planes of P: JT * 16 rows a block
+  const int jt = s <= 32 ? 2 : s <= 64 || s > 128 ? 4 : 8;
   const int jp = round_up(s, jt * 16), kp = round_up(s, 32);
+  Reach reach;
+  for (int i = 0; i < c.steps; ++i) reach.step(c.k);
+  const double by = UP * reach.hold();
   auto f64 = c.options.dtype(at::kDouble);
   auto part = at::empty({c.batch * chunks * size}, f64);
   auto pl = at::empty({2 * c.batch * jp * kp}, c.options.dtype(at::kHalf));
-  auto nm = at::empty({c.batch * 3}, c.options.dtype(at::kFloat));
+  auto nm = at::empty({c.batch * 2}, c.options.dtype(at::kFloat));
   _Float16* planes = (_Float16*)pl.data_ptr();
   Norm* norm = (Norm*)nm.data_ptr();
   double* parts = part.data_ptr<double>();
+  at::Tensor work;
   if (narrow) {
     auto go = [&](auto* gram, auto* chain, int threads) {
       hipLaunchKernelGGL(gram, dim3(chunks, c.batch), dim3(256), 0, c.stream,
                          parts, (const T*)c.u, c.touched, long_, s, chunk);
-      hipLaunchKernelGGL(chain, dim3(c.batch), dim3(threads), 0, c.stream, planes,
-                         norm, parts, c.touched, (int)chunks, s, c.steps, c.k,
-                         c.eps, jp, kp);
+      // one block would take longer over many parts than another kernel does
+      if (chunks * size > 131072) {
+        work = at::empty({c.batch * size}, f64);
+        hipLaunchKernelGGL(k_part_sum, dim3(size / 16, c.batch), dim3(256), 0,
+                           c.stream, work.data_ptr<double>(), parts,
+                           c.touched, (int)chunks, size);
+        parts = work.data_ptr<double>();
+        chunks = 1;
+      }
+      hipLaunchKernelGGL(chain, dim3(c.batch), dim3(threads), 0, c.stream,
+                         planes, norm, parts, c.touched, (int)chunks, s,
+                         c.steps, c.k, c.eps, jp, kp, by);
     };
     if (nt == 1) go(k_gram_narrow<T, TALL, 1>, k_chain<1, 4>, 256);
     else if (nt == 2) go(k_gram_narrow<T, TALL, 2>, k_chain<2, 16>, 1024);
     else go(k_gram_narrow<T, TALL, 4>, k_chain<4, 16>, 1024);
   } else {
     auto tr = at::empty({c.batch * chunks * super}, f64);
-    auto work = at::empty({6, c.batch * size}, f64);
+    work = at::empty({6, c.batch * size}, f64);
     double* w[6];
     for (int i = 0; i < 6; ++i)
       w[i] = work.data_ptr<double>() + i * c.batch * size;
     auto gram = [&](auto* kfn, const Momentum& q, const int64_t* place) {
-      hipLaunchKernelGGL(kfn, dim3(chunks, pairs, c.batch), dim3(256), 0,
+      hipLaunchKernelGGL(kfn, dim3(chunks, squares, c.batch), dim3(256), 0,
                          c.stream, parts, tr.data_ptr<double>(),
                          (const T*)c.u, q, place, c.touched, long_, s, sp,
                          chunk);
@@ -1418,20 +1501,23 @@ void run_thin(const Chain& c) {
       }
       if (i > 0) std::swap(p, p2);
     }
-    hipLaunchKernelGGL(k_small_out, dim3(c.batch), dim3(1024), 0, c.stream,
-                       planes, p, norm, c.touched, s, sp, jp, kp);
+    hipLaunchKernelGGL(k_small_out, dim3((jp * kp + 255) / 256, c.batch),
+                       dim3(256), 0, c.stream, planes, p, c.touched, s, sp, jp,
+                       kp, by);
   }
-  // turns of 128 places; a few a block where P's planes come in once
-  const int64_t turns = (long_ + 127) / 128;
-  const dim3 grid(std::min<int64_t>(turns, 2048), jp / (jt * 16), c.batch);
-  auto apply = [&](auto* kfn) {
-    hipLaunchKernelGGL(kfn, grid, dim3(256), 0, c.stream, c.res,
+  // a few turns a block, so that P's planes come in once for them
+  auto apply = [&](auto* kfn, int waves, int most) {
+    const int turn = waves * 16 * (TALL ? 2 : 4);
+    const dim3 grid(std::min<int64_t>((long_ + turn - 1) / turn, most),
+                    jp / (jt * 16), c.batch);
+    hipLaunchKernelGGL(kfn, grid, dim3(waves * WAVE), 0, c.stream, c.res,
                        (const T*)c.u, planes, norm, c.touched, long_, s, jp,
-                       kp);
+                       kp, (float)(1.0 / (UP * by)));
   };
-  if (jt == 2) apply(k_thin_apply<T, TALL, 2, 32>);
-  else if (jt == 4) apply(k_thin_apply<T, TALL, 4, 64>);
-  else apply(k_thin_apply<T, TALL, 8, 128>);
+  if (s <= 32) apply(k_thin_apply<T, TALL, 2, 32, 4>, 4, 2048);
+  else if (s <= 64) apply(k_thin_apply<T, TALL, 4, 64, 4>, 4, 2048);
+  else if (s <= 128) apply(k_thin_apply<T, TALL, 8, 128, 4>, 4, 2048);
+  else apply(k_thin_apply<T, TALL, 4, 320, 8>, 8, 256);
 }
 
 // Tiles of one product, and how many blocks share the sum of those after the
@@ -1488,30 +1574,6 @@ void run_product(const Chain& c, Product pr, const Cut& cut, int jobs = 1) {
   if (cut.tile == 128) go(k_product<128, 2, E, T>, k_join<128, E, T>);
   else go(k_product<64, 4, E, T>, k_join<64, E, T>);
 }
-
-// How far P's values can reach: its value at singular values from 0 to 1.
-struct Reach {
-  double x[257], p[257];
-  Reach() {
-    for (int i = 0; i < 257; ++i) {
-      x[i] = i / 256.0;
-      p[i] = 1.0;
-    }
-  }
-  void step(const Coeffs& k) {
-    for (int i = 0; i < 257; ++i) {
-      const double y = x[i] * x[i], q = k.a + k.b * y + k.c * y * y;
-      p[i] *= q;
-      x[i] *= q;
-    }
-  }
-  // the power of two that keeps P under 4, up to what lies between the points
-  float hold() const {
-    double top = 0;
-    for (double v : p) top = std::max(top, std::abs(v));
-    return top > 4 ? (float)std::exp2(-std::ceil(std::log2(top / 4))) : 1.0f;
-  }
-};
 
 // Whether all steps are taken on the Gram matrix, before P is applied to X.
 // With L = r s a step costs 3 r + 1 products of s^3 on X and about 4 on s x s

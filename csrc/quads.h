@@ -56,6 +56,19 @@ struct Quad {
   __device__ inline void set(int i, T t) { v[i] = *(Raw*)&t; }
 };
 
+// The same of two
+template <typename T>
+struct Pair {
+  using Raw = typename Bits<T>::Raw;
+  typedef Raw Vec __attribute__((ext_vector_type(2), aligned(sizeof(T))));
+  Vec v;
+  __device__ inline void load(const T* at) { v = *(const Vec*)at; }
+  __device__ inline T get(int i) const {
+    Raw r = v[i];
+    return *(T*)&r;
+  }
+};
+
 // The first `held` (any number) of four values, zeros after them.
 template <typename T>
 __device__ inline float4 load_quad(const T* at, int64_t held) {

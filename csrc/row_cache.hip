@@ -64,16 +64,27 @@ __device__ inline float scale_of(uint32_t amax_bits) {
   return __uint_as_float((uint32_t)(k + 127) << 23);
 }
 
-// Nearest integer to the exact quotient x / s, ties to even.  x * inv is off
-// by at most one step next to a half; the remainder x - q s is exact in one
-// fma (a multiple of ulp(s) / 2 no larger than s) and says which way.
-__device__ inline int code_int8(float x, float s, float inv) {
-  float q = rintf(x * inv);
-  float r = fmaf(-q, s, x);
-  float twice = 2.0f * fabsf(r);
-  bool odd = ((int)q) & 1;
-  if (twice > s || (twice == s && odd)) q += copysignf(1.0f, r);
-  return (int)q;
+// Nearest integer to the exact quotient x / s, ties to even, from q, which is
+// off by one at most: the remainder x - q s is exact in one fma (a multiple of
+// ulp(s) / 2 no larger than s) and says which way.
+__device__ inline float nearest(float q, float x, float s) {
+  const float r = fmaf(-q, s, x), twice = 2.0f * fabsf(r);
+  const bool odd = ((int)q) & 1;
+  return twice > s || (twice == s && odd) ? q + copysignf(1.0f, r) : q;
+}
+
+// x * inv is off the quotient by 2^-15 at most (128 steps of 2^-23 relative,
+// three roundings), so only values that near to a half need the remainder.
+__device__ inline uint32_t codes_int8(float4 f, float s, float inv) {
+  float4 y = make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
+  float4 q = make_float4(rintf(y.x), rintf(y.y), rintf(y.z), rintf(y.w));
+  const float off = fmaxf(fmaxf(fabsf(y.x - q.x), fabsf(y.y - q.y)),
+                          fmaxf(fabsf(y.z - q.z), fabsf(y.w - q.w)));
+  if (off > 0.4999f)
+    q = make_float4(nearest(q.x, f.x, s), nearest(q.y, f.y, s),
+                    nearest(q.z, f.z, s), nearest(q.w, f.w, s));
+  return (uint32_t)((int)q.x & 255) | (uint32_t)((int)q.y & 255) << 8 |
+         (uint32_t)((int)q.z & 255) << 16 | (uint32_t)(int)q.w << 24;
 }
 
 __device__ inline uint32_t quad_magnitude(float4 f) {
@@ -98,10 +109,7 @@ __device__ inline uint32_t encode(float4 f, float s, float inv) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(part(f.z), part(f.w), w,
                                                      true);
   }
-  return (uint32_t)(code_int8(f.x, s, inv) & 255) |
-         (uint32_t)(code_int8(f.y, s, inv) & 255) << 8 |
-         (uint32_t)(code_int8(f.z, s, inv) & 255) << 16 |
-         (uint32_t)code_int8(f.w, s, inv) << 24;
+  return codes_int8(f, s, inv);
 }
 
 template <bool FP8>
