@@ -1387,10 +1387,11 @@ bool is_thin(int64_t batch, int64_t m, int64_t n) {
 struct Reach {
   double x[257], p[257];
   Reach() {
-    for (int i = 0; i < 257; ++i) {
-      x[i] = i / 256.0;
-      p[i] = 1.0;
-    }
+    for (int i = 0; i < 257; ++i) x[i] = i / 256.0;
+    start();
+  }
+  void start() {
+    for (double& v : p) v = 1.0;
   }
   void step(const Coeffs& k) {
     for (int i = 0; i < 257; ++i) {
@@ -1575,17 +1576,20 @@ void run_product(const Chain& c, Product pr, const Cut& cut, int jobs = 1) {
   else go(k_product<64, 4, E, T>, k_join<64, E, T>);
 }
 
-// Whether all steps are taken on the Gram matrix, before P is applied to X.
-// With L = r s a step costs 3 r + 1 products of s^3 on X and about 4 on s x s
-// matrices, which need 3 r for G and P X once.  What G is off grows by a^2 with
-// every step and reaches a few parts in 10^4 of the result after five of Muon's:
-// below bfloat16's rounding, not below the others'; with more steps, which bring
-// up smaller singular values, it does not stay there.
+// How many steps in a row are taken on the Gram matrix before P is applied to
+// X; 1 for none.  With L = r s a step costs 3 r + 1 products of s^3 on X, and n
+// in a row cost 3 r + 4 n - 3.  What G is off grows by a^2 with every step: n is
+// bounded so that it does so by 200 in all (three of Muon's).  The result of
+// five is then a few parts in 10^5 off, whatever the singular values: far below
+// bfloat16's rounding, but several times what steps on X leave, so the other
+// types take those.
 template <typename T>
-bool by_gram(const Chain& c, int64_t s, int64_t long_) {
-  return std::is_same_v<T, __hip_bfloat16> && c.steps > 1 &&
-         long_ * 2 >= s * 3 &&
-         std::pow(c.k.a * c.k.a, c.steps - 1) <= 21000.0;
+int steps_on_gram(const Chain& c, int64_t s, int64_t long_) {
+  if (!std::is_same_v<T, __hip_bfloat16> || long_ * 2 < s * 3) return 1;
+  int n = 1;
+  double power = 1.0, sum = 1.0;
+  while (n < c.steps && (sum += power *= c.k.a * c.k.a) <= 200.0) ++n;
+  return n;
 }
 
 template <typename T>
@@ -1661,10 +1665,10 @@ void run_wide(const Chain& c) {
     std::swap(xt, xt2);
   };
 
-  new_gram();
-  if (!by_gram<T>(c, s, long_)) {
+  const int row = steps_on_gram<T>(c, s, long_);
+  if (row == 1) {
     for (int i = 0; i < c.steps; ++i) {
-      if (i) new_gram();
+      new_gram();
       new_poly(q);
       apply(q, 1.0f, i + 1 == c.steps);
     }
@@ -1673,30 +1677,36 @@ void run_wide(const Chain& c) {
   // Q from G; P <- P Q (the first P is Q); G <- Q (G Q)
   Planes p = square(), p2 = square(), t = square(), g2 = square();
   Reach reach;
-  float held = 1.0f;  // P's planes hold P times this
-  for (int i = 0; i < c.steps; ++i) {
-    const bool last = i + 1 == c.steps;
-    const Planes qi = i ? q : p;
-    new_poly(qi);
-    reach.step(c.k);
-    if (i) {
-      const float to = reach.hold();
-      pr.f[0] = {p, q, p2, down * (to / held)};
-      held = to;
-      pr.f[1] = {g, q, t, down};
-      run_product<GRAM, T>(c, pr, poly, last ? 1 : 2);
-      std::swap(p, p2);
-    } else {
-      pr.f[0] = {g, qi, t, down};
-      run_product<GRAM, T>(c, pr, poly);
+  for (int done = 0; done < c.steps;) {
+    const int todo = std::min(row, c.steps - done);
+    float held = 1.0f;  // P's planes hold P times this
+    reach.start();
+    new_gram();
+    for (int i = 0; i < todo; ++i) {
+      const bool last = i + 1 == todo;
+      const Planes qi = i ? q : p;
+      new_poly(qi);
+      reach.step(c.k);
+      if (i) {
+        const float to = reach.hold();
+        pr.f[0] = {p, q, p2, down * (to / held)};
+        held = to;
+        pr.f[1] = {g, q, t, down};
+        run_product<GRAM, T>(c, pr, poly, last ? 1 : 2);
+        std::swap(p, p2);
+      } else if (!last) {
+        pr.f[0] = {g, qi, t, down};
+        run_product<GRAM, T>(c, pr, poly);
+      }
+      if (!last) {
+        pr.f[0] = {qi, t, g2, down};
+        run_product<GRAM, T>(c, pr, poly);
+        std::swap(g, g2);
+      }
     }
-    if (!last) {
-      pr.f[0] = {qi, t, g2, down};
-      run_product<GRAM, T>(c, pr, poly);
-      std::swap(g, g2);
-    }
+    done += todo;
+    apply(p, held, done == c.steps);
   }
-  apply(p, held, true);
 }
 
 template <typename T>

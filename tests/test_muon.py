@@ -67,6 +67,9 @@ def matrices(kind, b, m, n, seed):
         left = torch.randn(b, m, r, generator=g)
         left /= torch.arange(1, r + 1)
         x = torch.bmm(left, torch.randn(b, r, n, generator=g)) + 0.05 * x
+    if kind == "steep":  # four directions a thousand times the others
+        x = 1e-3 * x + torch.bmm(torch.randn(b, m, 4, generator=g),
+                                 torch.randn(b, 4, n, generator=g))
     return x
 
 
@@ -111,7 +114,7 @@ def test_16_bit_types(device, dtype, m, n):
 
 
 @pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("kind", ["normal", "decay"])
+@pytest.mark.parametrize("kind", ["normal", "decay", "steep"])
 @pytest.mark.parametrize("steps,coeffs", [(1, ops.MUON_COEFFS),
                                           (2, ops.MUON_COEFFS),
                                           (5, ops.MUON_COEFFS),
@@ -122,15 +125,16 @@ def test_16_bit_types(device, dtype, m, n):
 @pytest.mark.parametrize("m,n", [(140, 300), (300, 140), (130, 2100),
                                  (520, 790)])
 def test_long_bfloat16_matrices(device, kind, steps, coeffs, m, n):
-    """The steps may be taken on the Gram matrix where that stays below
-    bfloat16's rounding: the error of the result is at most half as much
-    again as that of the exact result's rounding."""
+    """Some steps in a row may be taken on the Gram matrix where that stays
+    below bfloat16's rounding, also where a few singular values are a thousand
+    times the others: the error of the result is at most a tenth more than
+    that of the exact result's rounding."""
     x = matrices(kind, 2, m, n, 12).bfloat16()
     got = ops.orthogonalize(x.to(device), steps=steps, coeffs=coeffs).cpu()
     for k in range(2):
         want, _ = chain(x[k], steps=steps, coeffs=coeffs)
         rounding = float((want.bfloat16().double() - want).norm())
-        assert float((got[k].double() - want).norm()) <= 1.5 * rounding
+        assert float((got[k].double() - want).norm()) <= 1.1 * rounding
 
 
 @pytest.mark.parametrize("device", DEVICES)
