@@ -22,6 +22,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "ops.h"
@@ -51,17 +52,28 @@ __device__ inline uint32_t magnitude(float x) {
   return __float_as_uint(x) & 0x7fffffffu;
 }
 
+struct Scale { float s, inv; };  // inv is 1 / s: fp8 exactly, int8 nearly
+
 template <bool FP8>
-__device__ inline float scale_of(uint32_t amax_bits) {
-  if (amax_bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
-  float amax = __uint_as_float(amax_bits);
-  if (!FP8) return fminf(fmaxf(amax / 127.0f, TINY), INT8_TOP);
+__device__ inline Scale scale_of(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.0f};
+  const float amax = __uint_as_float(amax_bits);
+  if (!FP8) {
+    // amax / 127: the product with the rounded reciprocal is off by an ulp at
+    // most, its remainder is exact, and one fma rounds the sum correctly
+    constexpr float y = 1.0f / 127.0f;
+    const float q = amax * y;
+    const float s = fminf(fmaxf(fmaf(fmaf(-127.0f, q, amax), y, q), TINY),
+                          INT8_TOP);
+    return {s, __builtin_amdgcn_rcpf(s)};
+  }
   // 448 = 1.75 * 2^8: with amax = m * 2^e, 1 <= m < 2, the exponent is
   // e - 8 while m <= 1.75 and e - 7 above.  (Subnormal: the 2^-126 floor.)
   int e = (int)(amax_bits >> 23) - 127;
   int k = (amax_bits & 0x7fffffu) <= 0x600000u ? e - 8 : e - 7;
   if (k < -126) k = -126;
-  return __uint_as_float((uint32_t)(k + 127) << 23);
+  return {__uint_as_float((uint32_t)(k + 127) << 23),
+          __uint_as_float((uint32_t)(127 - k) << 23)};
 }
 
 // Nearest integer to the exact quotient x / s, ties to even, from q, which is
@@ -73,8 +85,9 @@ __device__ inline float nearest(float q, float x, float s) {
   return twice > s || (twice == s && odd) ? q + copysignf(1.0f, r) : q;
 }
 
-// x * inv is off the quotient by 2^-15 at most (128 steps of 2^-23 relative,
-// three roundings), so only values that near to a half need the remainder.
+// x * inv is off the quotient by 2^-15 at most (inv by an ulp, the product by
+// half of one, 2^7 steps), so only values that near to a half need the
+// remainder.
 __device__ inline uint32_t codes_int8(float4 f, float s, float inv) {
   float4 y = make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
   float4 q = make_float4(rintf(y.x), rintf(y.y), rintf(y.z), rintf(y.w));
@@ -99,7 +112,8 @@ __device__ inline uint32_t group_max(uint32_t v, int group) {
 }
 
 template <bool FP8>
-__device__ inline uint32_t encode(float4 f, float s, float inv) {
+__device__ inline uint32_t encode(float4 f, Scale sc) {
+  const float s = sc.s, inv = sc.inv;
   if (s != s) return 0;  // the row is not finite
   if (FP8) {
     auto part = [&](float x) {
@@ -173,16 +187,15 @@ __global__ __launch_bounds__(256) void k_cache_write(
       uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < QUADS; ++i) top = max(top, quad_magnitude(x[r][i]));
-      const float s = scale_of<FP8>(group_max(top, group));
-      const float inv = 1.0f / s;
+      const Scale s = scale_of<FP8>(group_max(top, group));
       if (slot[r] < 0) continue;
       uint32_t* out = (uint32_t*)(cache + slot[r] * cache_stride);
 #pragma unroll
       for (int i = 0; i < QUADS; ++i) {
         const int q = lane + i * group;
-        if (q < quads) out[q] = encode<FP8>(x[r][i], s, inv);
+        if (q < quads) out[q] = encode<FP8>(x[r][i], s);
       }
-      if (lane == 0) out[quads] = __float_as_uint(s);
+      if (lane == 0) out[quads] = __float_as_uint(s.s);
     }
   }
 }
@@ -205,11 +218,10 @@ __global__ __launch_bounds__(256) void k_cache_write_long(
     uint32_t top = 0;
     for (int64_t q = lane; q < quads; q += WAVE)
       top = max(top, quad_magnitude(load_quad(x + q * 4, dim - q * 4)));
-    const float s = scale_of<FP8>(group_max(top, WAVE));
-    const float inv = 1.0f / s;
+    const Scale s = scale_of<FP8>(group_max(top, WAVE));
     for (int64_t q = lane; q < quads; q += WAVE)
-      out[q] = encode<FP8>(load_quad(x + q * 4, dim - q * 4), s, inv);
-    if (lane == 0) out[quads] = __float_as_uint(s);
+      out[q] = encode<FP8>(load_quad(x + q * 4, dim - q * 4), s);
+    if (lane == 0) out[quads] = __float_as_uint(s.s);
   }
 }
 
@@ -280,18 +292,48 @@ int grid_of(int64_t blocks) {
 }
 
 // How lanes share a row: `group` lanes of `quads` quads each, 0 quads for a
-// row too long for registers.
+// row too long for registers.  The pair that leaves the fewest places of it
+// empty, under 32 lanes only if it saves a fifth; of several, up to four quads
+// and lanes near to 32 (500,000 x 256 bf16 as fp8: 32 x 2 4.6 TB/s, 64 x 1 3.8;
+// 1,000,000 x 300 f32 as int8: 16 x 5 4% slower than 32 x 3; 100,003 x 77 f16:
+// 8 x 3 10 us, 32 x 1 16.5).
 struct Share { int group, quads; };
 
 Share share_of(int64_t dim) {
   const int64_t need = (dim + 3) / 4;
   if (need > WAVE * 8) return {WAVE, 0};
-  int group = 1, quads = 1;
-  while (group < 32 && group < need) group *= 2;
-  while (group * quads < need && quads < 4) quads *= 2;
-  while (group * quads < need && group < WAVE) group *= 2;
-  while (group * quads < need) quads *= 2;
-  return {group, quads};
+  Share best{0, 0};
+  int least = INT_MAX;
+  for (int group : {32, 64, 16, 8, 4, 2, 1}) {
+    if (group < 8 && need > 4) break;
+    const int64_t q = (need + group - 1) / group;
+    const int quads = q == 7 ? 8 : (int)q;
+    const int cost = group * quads * (group < 32 ? 5 : 4);
+    if (quads <= 8 && (cost < least ||
+                       (cost == least && best.quads > 4 && quads <= 4))) {
+      best = {group, quads};
+      least = cost;
+    }
+  }
+  return best;
+}
+
+// f(std::integral_constant<QUADS>{}, std::integral_constant<ROWS>{})
+template <typename F>
+void by_share(int quads, F f) {
+  using std::integral_constant;
+  if (quads == 1) f(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+  else if (quads == 2)
+    f(integral_constant<int, 2>{}, integral_constant<int, 2>{});
+  else if (quads == 3)
+    f(integral_constant<int, 3>{}, integral_constant<int, 2>{});
+  else if (quads == 4)
+    f(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+  else if (quads == 5)
+    f(integral_constant<int, 5>{}, integral_constant<int, 1>{});
+  else if (quads == 6)
+    f(integral_constant<int, 6>{}, integral_constant<int, 1>{});
+  else f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
 }
 
 template <typename T, bool FP8>
@@ -307,10 +349,11 @@ void launch_write(at::Tensor& cache, const at::Tensor& values, Slots slots,
                        stream, out, cache.stride(0), x, values.stride(0),
                        slots, owner, n, (int)dim, cache.size(0), sh.group);
   };
-  if (sh.quads == 1) go(k_cache_write<T, FP8, 1, 4>, 4);
-  else if (sh.quads == 2) go(k_cache_write<T, FP8, 2, 2>, 2);
-  else if (sh.quads == 4) go(k_cache_write<T, FP8, 4, 1>, 1);
-  else if (sh.quads == 8) go(k_cache_write<T, FP8, 8, 1>, 1);
+  if (sh.quads)
+    by_share(sh.quads, [&](auto q, auto r) {
+      constexpr int Q = decltype(q)::value, R = decltype(r)::value;
+      go(k_cache_write<T, FP8, Q, R>, R);
+    });
   else
     hipLaunchKernelGGL((k_cache_write_long<T, FP8>), dim3(grid_of((n + 3) / 4)),
                        dim3(256), 0, stream, out, cache.stride(0), x,
@@ -330,10 +373,11 @@ void launch_read(at::Tensor& out, const at::Tensor& cache, Slots slots,
                        stream, to, from, cache.stride(0), slots, n, (int)dim,
                        cache.size(0), sh.group);
   };
-  if (sh.quads == 1) go(k_cache_read<T, FP8, 1, 4>, 4);
-  else if (sh.quads == 2) go(k_cache_read<T, FP8, 2, 2>, 2);
-  else if (sh.quads == 4) go(k_cache_read<T, FP8, 4, 1>, 1);
-  else if (sh.quads == 8) go(k_cache_read<T, FP8, 8, 1>, 1);
+  if (sh.quads)
+    by_share(sh.quads, [&](auto q, auto r) {
+      constexpr int Q = decltype(q)::value, R = decltype(r)::value;
+      go(k_cache_read<T, FP8, Q, R>, R);
+    });
   else
     hipLaunchKernelGGL((k_cache_read_long<T, FP8>), dim3(grid_of((n + 3) / 4)),
                        dim3(256), 0, stream, to, from, cache.stride(0), slots,
