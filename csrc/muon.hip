@@ -255,6 +255,9 @@ __device__ inline double2 norm_factors(double sumsq, double eps) {
 }
 
 __device__ inline void split(float v, _Float16& hi, _Float16& lo) {
+  // v as it is: a product that the compiler fuses with one of the conversions
+  // and not with the other gives them two values of hi, once in 2^14
+  asm("" : "+v"(v));
   hi = (_Float16)v;
   lo = (_Float16)(v - (float)hi);
 }
