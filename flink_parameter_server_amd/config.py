@@ -46,7 +46,8 @@ class PSConfig:
 
     # Wire dtype for pull answers / push deltas: "f32", "bf16", or 8-bit
     # row records with one f32 scale a row, "int8" (steps of the row's
-    # largest magnitude / 127) or "fp8" (e4m3; ops.cache_write).
+    # largest magnitude / 127) or "e4m3" (8-bit floats; the format that
+    # ops.cache_write calls "fp8").
     # Tables always keep f32 master values.
     wire_dtype: str = "f32"
 
@@ -89,7 +90,7 @@ class PSConfig:
             raise ValueError("n_workers and n_shards must be >= 1")
         if self.partitioner not in ("mod", "range"):
             raise ValueError(f"unknown partitioner {self.partitioner!r}")
-        if self.wire_dtype not in ("f32", "bf16", "int8", "fp8"):
+        if self.wire_dtype not in ("f32", "bf16", "int8", "e4m3"):
             raise ValueError(f"unknown wire_dtype {self.wire_dtype!r}")
         if self.feedback not in ("fresh", "merged", "pipelined"):
             raise ValueError(f"unknown feedback {self.feedback!r}")

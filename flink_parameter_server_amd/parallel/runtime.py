@@ -54,6 +54,9 @@ from ..config import PSConfig
 from .partitioner import Partitioner, bucket_by_shard, make_partitioner
 from .transport import Transport, LocalTransport
 
+#: wire dtypes that are 8-bit row records -> their row format
+_RECORD_FORMATS = {"int8": "int8", "e4m3": "fp8"}
+
 
 @dataclass
 class Metrics:
@@ -703,10 +706,10 @@ class PSEngine:
 
     def _wire_spec(self) -> Tuple[torch.dtype, Tuple[int, ...]]:
         """(dtype, trailing shape) of a payload row on the wire."""
-        fmt, dim = self.cfg.wire_dtype, self.cfg.dim
-        if fmt in ("int8", "fp8"):
+        wire, dim = self.cfg.wire_dtype, self.cfg.dim
+        if wire in _RECORD_FORMATS:
             return torch.uint8, (ops.record_bytes(dim),)
-        return (torch.bfloat16 if fmt == "bf16" else torch.float32), (dim,)
+        return (torch.bfloat16 if wire == "bf16" else torch.float32), (dim,)
 
     def _wire_out(self, chan: List[Optional[torch.Tensor]]) -> None:
         """Narrow a payload channel to the wire dtype in place (bf16 halves
@@ -714,29 +717,28 @@ class PSEngine:
         masters, so only the wire narrows).
         The self-addressed segment short-circuits in every transport and
         stays f32 — full precision for the 1/world local fraction."""
-        fmt = self.cfg.wire_dtype
-        if fmt == "f32":
+        wire = self.cfg.wire_dtype
+        if wire == "f32":
             return
         for d, t in enumerate(chan):
             if t is None or d == self.rank:
                 continue
-            if fmt == "bf16":
+            if wire == "bf16":
                 chan[d] = t.to(torch.bfloat16)
             else:
                 t = t.detach().reshape(-1, self.cfg.dim).float()
                 rec = torch.empty(t.shape[0], ops.record_bytes(self.cfg.dim),
                                   dtype=torch.uint8, device=t.device)
-                ops.cache_write(rec, t, fmt=fmt)
+                ops.cache_write(rec, t, fmt=_RECORD_FORMATS[wire])
                 chan[d] = rec
 
     def _unwire(self, chan: List[Optional[torch.Tensor]]) -> None:
-        records = self.cfg.wire_dtype in ("int8", "fp8")
+        fmt = _RECORD_FORMATS.get(self.cfg.wire_dtype)
         for s, t in enumerate(chan):
             if t is None or t.dtype is torch.float32:
                 continue
-            if records and s != self.rank:
-                chan[s] = ops.cache_read(t, self.cfg.dim,
-                                         fmt=self.cfg.wire_dtype)
+            if fmt is not None and s != self.rank:
+                chan[s] = ops.cache_read(t, self.cfg.dim, fmt=fmt)
             else:
                 chan[s] = t.float()
 
