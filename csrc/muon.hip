@@ -177,11 +177,13 @@ __global__ __launch_bounds__(256) void k_places(
     }
     touched[b] = some;
   }
-  for (int64_t j = lo + threadIdx.x; j < hi; j += 256)
-    if (j == lo || rows[j - 1] != rows[j])
-      mine[rows[j] - r0] = j + 1 < hi && rows[j + 1] == rows[j]
-                               ? several(j)
-                               : (order ? order[j] : j);
+  for (int64_t j = lo + threadIdx.x; j < hi; j += 256) {
+    const int64_t at = rows[j] - r0;  // within, unless rows are not sorted
+    if (at >= 0 && at < count && (j == lo || rows[j - 1] != rows[j]))
+      mine[at] = j + 1 < hi && rows[j + 1] == rows[j]
+                     ? several(j)
+                     : (order ? order[j] : j);
+  }
   __syncthreads();
   if (threadIdx.x < count) place[r0 + threadIdx.x] = mine[threadIdx.x];
 }
@@ -247,8 +249,10 @@ struct Norm { float x, y; };
 // X = U / n with n = |U|_F + eps as (u x) y: the power of two x keeps y and
 // the products normal for values near the ends of f32's range.  NaN for a
 // matrix that is not finite.
+// eps < 0: U is X already.
 __device__ inline double2 norm_factors(double sumsq, double eps) {
   if (!(sumsq < INFINITY)) return make_double2(1.0, NAN);
+  if (eps < 0) return make_double2(1.0, 1.0);
   const double n = sqrt(sumsq) + eps;
   const double x = n > 0x1p60 ? 0x1p-60 : (n < 0x1p-60 ? 0x1p60 : 1.0);
   return make_double2(x, 1.0 / (n * x));
@@ -1396,12 +1400,16 @@ struct Reach {
   void start() {
     for (double& v : p) v = 1.0;
   }
-  void step(const Coeffs& k) {
+  // a step; how much it multiplies by at most
+  double step(const Coeffs& k) {
+    double top = 0;
     for (int i = 0; i < 257; ++i) {
       const double y = x[i] * x[i], q = k.a + k.b * y + k.c * y * y;
       p[i] *= q;
       x[i] *= q;
+      top = std::max(top, std::abs(q));
     }
+    return top;
   }
   // the power of two that keeps P under 4, up to what lies between the points
   float hold() const {
@@ -1581,7 +1589,7 @@ void run_product(const Chain& c, Product pr, const Cut& cut, int jobs = 1) {
 
 // How many steps in a row are taken on the Gram matrix before P is applied to
 // X; 1 for none.  With L = r s a step costs 3 r + 1 products of s^3 on X, and n
-// in a row cost 3 r + 4 n - 3.  What G is off grows by a^2 with every step: n is
+// in a row cost 3 r + 4 n - 3.  What G is off grows by q^2 with every step: n is
 // bounded so that it does so by 200 in all (three of Muon's).  The result of
 // five is then a few parts in 10^5 off, whatever the singular values: far below
 // bfloat16's rounding, but several times what steps on X leave, so the other
@@ -1589,10 +1597,14 @@ void run_product(const Chain& c, Product pr, const Cut& cut, int jobs = 1) {
 template <typename T>
 int steps_on_gram(const Chain& c, int64_t s, int64_t long_) {
   if (!std::is_same_v<T, __hip_bfloat16> || long_ * 2 < s * 3) return 1;
-  int n = 1;
-  double power = 1.0, sum = 1.0;
-  while (n < c.steps && (sum += power *= c.k.a * c.k.a) <= 200.0) ++n;
-  return n;
+  Reach reach;
+  int n = 0;
+  for (double power = 1.0, sum = 0.0; n < c.steps; ++n) {
+    if ((sum += power) > 200.0) break;
+    const double q = reach.step(c.k);
+    power *= q * q;
+  }
+  return std::max(n, 1);
 }
 
 template <typename T>
@@ -1713,11 +1725,53 @@ void run_wide(const Chain& c) {
 }
 
 template <typename T>
+void thin(const Chain& c) {
+  if (c.m >= c.n) run_thin<T, true>(c); else run_thin<T, false>(c);
+}
+
+// P's planes hold 40 bits from its largest value down, and the values that
+// matter are near one: steps are taken in one round while P does not reach
+// beyond 2^11 (six of Muon's).
+int thin_round(const Coeffs& k, int steps) {
+  Reach reach;
+  int n = 0;
+  while (n < steps) {
+    reach.step(k);
+    if (n && reach.hold() < 0x1p-9f) break;
+    ++n;
+  }
+  return n;
+}
+
+template <typename T>
 void run(const Chain& c) {
-  if (is_thin(c.batch, c.m, c.n)) {
-    if (c.m >= c.n) run_thin<T, true>(c); else run_thin<T, false>(c);
-  } else {
+  if (!is_thin(c.batch, c.m, c.n)) {
     run_wide<T>(c);
+    return;
+  }
+  const int most = thin_round(c.k, c.steps);
+  if (most == c.steps) {
+    thin<T>(c);
+    return;
+  }
+  // several rounds, with X in f32 between
+  TORCH_CHECK((std::is_same_v<T, float>), "rounds are taken in f32");
+  Chain round = c;
+  at::Tensor x, next;
+  for (int done = 0; done < c.steps; done += most) {
+    round.steps = std::min(most, c.steps - done);
+    next = at::Tensor();
+    if (done + most < c.steps) {
+      next = at::empty({c.batch * c.m * c.n}, c.options.dtype(at::kFloat));
+      round.res = {next.data_ptr(), 0, 0, false};
+    } else {
+      round.res = c.res;
+    }
+    thin<T>(round);
+    x = next;
+    if (x.defined()) round.u = x.data_ptr();
+    round.fused = false;
+    round.eps = -1.0;  // U is X already
   }
 }
 
@@ -1766,6 +1820,9 @@ at::Tensor orthogonalize(at::Tensor x, int64_t steps, double a, double b,
   c10::DeviceGuard guard(x.device());
   auto out = at::empty_like(x);
   if (!x.numel()) return out;
+  if (type != at::kFloat && is_thin(x.size(0), x.size(1), x.size(2)) &&
+      thin_round({a, b, c}, steps) < steps)
+    return orthogonalize(x.to(at::kFloat), steps, a, b, c, eps).to(type);
   dispatch(Chain{x.data_ptr(), type, x.size(0), x.size(1), x.size(2), nullptr,
                  nullptr, (int)steps, {a, b, c}, eps, {out.data_ptr(), 0, 0, false},
                  x.options(), at::hip::getCurrentHIPStream().stream()});

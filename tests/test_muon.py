@@ -104,6 +104,26 @@ def test_orthogonalize_large(b, m, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("steps", [6, 7, 12, 13, 20, 100])
+@pytest.mark.parametrize("m,n", [(24, 40), (2000, 40), (600, 128),
+                                 (128, 600), (9000, 200), (150, 170)])
+def test_many_steps(m, n, steps, dtype):
+    """However often steps multiply what is small, the result stays near the
+    one in 64 bits: at most eight times as far as the oracle's f32 steps are
+    (which keep every value in f32 and round as often)."""
+    x = matrices("normal", 1, m, n, 14).to(dtype)
+    want = chain(x[0], steps=steps)[0]
+    got = ops.orthogonalize(x.cuda(), steps=steps).cpu()
+    f32 = ops.orthogonalize(x.float(), steps=steps)
+    limit = 8 * float((f32[0].double() - want).norm())
+    if dtype != torch.float32:
+        limit += torch.finfo(dtype).eps / 2 * float(want.norm())
+    off = float((got[0].double() - want).norm())
+    assert off <= limit
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m,n", [(6040, 32), (32, 6040), (4000, 60),
                                  (20000, 100), (100, 20000), (9000, 200),
                                  (700, 600), (600, 700)])
@@ -147,7 +167,8 @@ def test_long_bfloat16_matrices(device, kind, steps, coeffs, m, n):
     for k in range(2):
         want, _ = chain(x[k], steps=steps, coeffs=coeffs)
         rounding = float((want.bfloat16().double() - want).norm())
-        assert float((got[k].double() - want).norm()) <= 1.1 * rounding
+        off = float((got[k].double() - want).norm())
+        assert off <= 1.1 * rounding
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -343,6 +364,39 @@ def test_apply_muon_orders_and_index_types(device):
     assert torch.equal(five[0], table) and int(five[1].abs().sum()) == 0
     six = step(rows[:0], grads[:0])
     assert torch.equal(six[0], table)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(300, 20), (700, 100)])
+def test_apply_muon_many_steps(m, n):
+    """The step's rounds end in the table, from the momentum's own pass."""
+    g = torch.randn(m, n)
+    table, mo = torch.randn(m, n), torch.randn(m, n)
+    rows = torch.arange(m)
+    t, v = table.cuda(), mo.cuda()
+    ops.apply_muon(t, v, rows.cuda(), g.cuda(), 0.1, steps=9,
+                   sorted_unique=True)
+    M = 0.95 * mo.double() + g.double()
+    step = ops.orthogonalize((g.double() + 0.95 * M).float(), steps=9)
+    want = table.double() - 0.1 * math.sqrt(m / n) * step.double()
+    # two f32 chains of nine steps, each off by at most `chain`'s bound
+    limit = 2 * 0.1 * math.sqrt(m / n) * chain(g + 0.95 * M, steps=9)[1]
+    off = float((t.cpu().double() - want).norm())
+    assert off <= limit
+    # near enough to say that no step is missing: one changes values by a
+    # fifth of their size and more
+    assert off <= 1e-3 * float((want - table.double()).norm())
+
+
+@pytest.mark.gpu
+def test_rows_that_are_not_sorted_as_promised_stay_inside():
+    """A broken promise gives wrong sums, not a fault."""
+    table = torch.randn(600, 8, device="cuda")
+    mo = torch.zeros_like(table)
+    rows = torch.randint(-5, 700, (900,), device="cuda")
+    ops.apply_muon(table, mo, rows, torch.randn(900, 8, device="cuda"), 0.1,
+                   matrix_rows=300, sorted_unique=True)
+    assert bool(torch.isfinite(table).all())
 
 
 @pytest.mark.parametrize("device", DEVICES)
