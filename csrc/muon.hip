@@ -854,8 +854,10 @@ __global__ __launch_bounds__(WAVES * WAVE) void k_chain(
 // O = U P (TALL) or P U: 16 JT of P's rows, up to KS places long, in LDS; a wave
 // takes its values from memory to the matrix instructions by itself, split in
 // two planes on the way, CH places of the sum at a time.  A lane holds eight
-// places of long-axis row lane % 16 (TALL: its neighbours in memory), or of
-// four neighbouring ones, which lie in four tiles.  Bound by memory.
+// places of long-axis row lane % 16, or (wide) of four neighbouring ones, which
+// lie in four tiles.  Of 32 places of the sum, lane group g = lane / 16 takes
+// 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3, so that a load of four groups is
+// 64 bytes of a row; P lies in LDS in that order.  Bound by memory.
 template <typename T, bool TALL, int JT, int KS, int WAVES>
 __global__ __launch_bounds__(WAVES * WAVE) void k_thin_apply(
     Result res, const T* __restrict__ u, const _Float16* __restrict__ planes,
@@ -880,7 +882,10 @@ __global__ __launch_bounds__(WAVES * WAVE) void k_thin_apply(
     const int c = e % (KS / 8) * 8;
     half8 v = {};
     if (c < kp) v = *(const half8*)(p + h * plane + (int64_t)r * kp + c);
-    *(half8*)&lds[h][r * LP + c] = v;
+    // places c .. c + 3 are those of group c % 16 / 4, the next four the next's
+    _Float16* to = &lds[h][r * LP + c / 32 * 32 + c % 16 * 2 + c % 32 / 16 * 4];
+    *(half4*)to = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+    *(half4*)(to + 8) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
   }
   __syncthreads();
 
@@ -898,14 +903,14 @@ __global__ __launch_bounds__(WAVES * WAVE) void k_thin_apply(
       float raw[CH / 32][RT][8];
 #pragma unroll
       for (int ks = 0; ks < CH / 32; ++ks) {
-        const int k = kc + ks * 32 + lane / 16 * 8;
+        const int k = kc + ks * 32 + lane / 16 * 4;
         if (TALL) {
 #pragma unroll
           for (int w = 0; w < RT; ++w)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float4 f = load_quad(x + at(w) * s + k + h * 4,
-                                         at(w) < long_ ? s - k - h * 4 : 0);
+              const float4 f = load_quad(x + at(w) * s + k + h * 16,
+                                         at(w) < long_ ? s - k - h * 16 : 0);
               raw[ks][w][h * 4] = f.x;
               raw[ks][w][h * 4 + 1] = f.y;
               raw[ks][w][h * 4 + 2] = f.z;
@@ -914,8 +919,9 @@ __global__ __launch_bounds__(WAVES * WAVE) void k_thin_apply(
         } else {
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
-            const float4 f = load_quad(x + (k + c) * long_ + r0,
-                                       k + c < s ? long_ - r0 : 0);
+            const int kk = k + c % 4 + c / 4 * 16;
+            const float4 f = load_quad(x + kk * long_ + r0,
+                                       kk < s ? long_ - r0 : 0);
             raw[ks][0][c] = f.x;
             raw[ks][1][c] = f.y;
             raw[ks][2 % RT][c] = f.z;
