@@ -1110,13 +1110,41 @@ __device__ inline void tile_of(int t, int ns, int nl, int* bi, int* bj) {
   }
 }
 
+// a's values (both planes) that POLY adds, as a lane holds D's.
+template <int NT>
+struct Old {
+  half4 v[NT / 32][NT / 32][2];
+
+  __device__ inline void load(const Planes& a, int64_t b, int bi, int bj) {
+    const int lane = threadIdx.x % WAVE, wave = this_wave();
+    // a is symmetric: its row j has a lane's four values side by side
+    const _Float16* g =
+        a.p + b * a.batch +
+        ((int64_t)bj * NT + wave % 2 * (NT / 2) + lane % 16) * a.pitch +
+        (int64_t)bi * NT + wave / 2 * (NT / 2) + lane / 16 * 4;
+#pragma unroll
+    for (int ti = 0; ti < NT / 32; ++ti)
+#pragma unroll
+      for (int tj = 0; tj < NT / 32; ++tj)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          v[ti][tj][h] =
+              *(const half4*)(g + h * a.plane + tj * 16 * a.pitch + ti * 16);
+  }
+};
+
+// Halves of LDS that end_product needs.
+template <int NT>
+constexpr int end_size() { return 2 * NT * (NT + 8); }
+
 // What one block leaves of its tile: a lane holds D[i .. i + 3][j] of each
-// 16 x 16 tile of its wave's quarter.  `lds` is free to be written.
+// 16 x 16 tile of its wave's quarter.  `lds` is free to be written once
+// everybody is here.
 template <int NT, Ending E, typename T>
 __device__ inline void end_product(const Product& pr, const Factors& f,
                                    int64_t b, int bi, int bj,
                                    f32x4 (&acc)[NT / 32][NT / 32],
-                                   _Float16* lds) {
+                                   const Old<NT>& old, _Float16* lds) {
   constexpr int W = NT / 32;
   const int lane = threadIdx.x % WAVE, wave = this_wave();
   const int wi = wave / 2 * (NT / 2), wj = wave % 2 * (NT / 2);
@@ -1145,51 +1173,47 @@ __device__ inline void end_product(const Product& pr, const Factors& f,
   // D as it is goes out through LDS, in 16-byte pieces; D transposed, four
   // values a lane, from the registers.
   constexpr int ROW = NT + 8;
+  const bool both = E == UPDATE || bi != bj;
+  const Planes& t = E == UPDATE ? pr.dt : f.d;
+  __syncthreads();
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    __syncthreads();
+  for (int ti = 0; ti < W; ++ti)
 #pragma unroll
-    for (int ti = 0; ti < W; ++ti)
+    for (int tj = 0; tj < W; ++tj) {
+      const int li = wi + ti * 16 + lane / 16 * 4;
+      const int lj = wj + tj * 16 + lane % 16;
+      const int64_t i = (int64_t)bi * NT + li, j = (int64_t)bj * NT + lj;
+      const f32x4 v = acc[ti][tj] * f.scale;
+      half4 hi, lo;
 #pragma unroll
-      for (int tj = 0; tj < W; ++tj) {
-        const int li = wi + ti * 16 + lane / 16 * 4;
-        const int lj = wj + tj * 16 + lane % 16;
-        const int64_t i = (int64_t)bi * NT + li, j = (int64_t)bj * NT + lj;
-        if (h == 0) {
-          f32x4 v = acc[ti][tj] * f.scale;
-          if (E == POLY) {
-            // a is symmetric: its row j has the four values side by side
-            const _Float16* g = f.a.p + b * f.a.batch + j * f.a.pitch + i;
-            const half4 gh = *(const half4*)g;
-            const half4 gl = *(const half4*)(g + f.a.plane);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              v[r] = pr.cc * v[r] + pr.cb * ((float)gh[r] + (float)gl[r]);
-              if (i + r == j && j < pr.s) v[r] += pr.ca * UP;
-            }
-          }
-          acc[ti][tj] = v;
+      for (int r = 0; r < 4; ++r) {
+        float x = v[r];
+        if (E == POLY) {
+          x = pr.cc * x + pr.cb * ((float)old.v[ti][tj][0][r] +
+                                   (float)old.v[ti][tj][1][r]);
+          if (i + r == j && j < pr.s) x += pr.ca * UP;
         }
-        half4 w;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          _Float16 hi, lo;
-          split(acc[ti][tj][r], hi, lo);
-          w[r] = h ? lo : hi;
-          lds[(li + r) * ROW + lj] = w[r];
-        }
-        if (E == UPDATE || bi != bj) {
-          const Planes& t = E == UPDATE ? pr.dt : f.d;
-          *(half4*)(t.p + h * t.plane + b * t.batch + j * t.pitch + i) = w;
-        }
+        _Float16 xh, xl;
+        split(x, xh, xl);
+        hi[r] = xh;
+        lo[r] = xl;
+        lds[(li + r) * ROW + lj] = xh;
+        lds[(NT + li + r) * ROW + lj] = xl;
       }
-    __syncthreads();
-    for (int e = threadIdx.x; e < NT * NT / 8; e += 256) {
-      const int r = e / (NT / 8), c = e % (NT / 8) * 8;
-      *(half8*)(f.d.p + h * f.d.plane + b * f.d.batch +
-                ((int64_t)bi * NT + r) * f.d.pitch + (int64_t)bj * NT + c) =
-          *(const half8*)(lds + r * ROW + c);
+      if (both) {
+        _Float16* to = t.p + b * t.batch + j * t.pitch + i;
+        *(half4*)to = hi;
+        *(half4*)(to + t.plane) = lo;
+      }
     }
+  __syncthreads();
+#pragma unroll
+  for (int e = threadIdx.x; e < NT * NT / 4; e += 256) {
+    const int r = e / (NT / 8), c = e % (NT / 8) * 8;  // rows of both planes
+    const int h = r >= NT;
+    *(half8*)(f.d.p + h * f.d.plane + b * f.d.batch +
+              ((int64_t)bi * NT + r - h * NT) * f.d.pitch + (int64_t)bj * NT +
+              c) = *(const half8*)(lds + r * ROW + c);
   }
 }
 
@@ -1206,8 +1230,14 @@ __global__ __launch_bounds__(256, 2) void k_product(
   constexpr bool HALF = E == GRAM || E == POLY;
   constexpr int W = NT / 32;           // 16-tiles a wave on each side
   constexpr int LOADS = NT / 64;       // pieces a thread, operand and plane
-  __shared__ half8 lds[BUFFERS][2][2][NT * 4];  // buffer, operand, plane
-  static_assert(NT * (NT + 8) * sizeof(_Float16) <= sizeof(lds), "");
+  constexpr int PIECES = NT * 4;       // of an operand's plane
+  constexpr int STAGE = BUFFERS * 4 * PIECES, LAST = end_size<NT>() / 8;
+  __shared__ half8 lds[STAGE > LAST ? STAGE : LAST];
+  auto stage = [&](int buffer, int operand, int h) {
+    return lds + ((buffer * 2 + operand) * 2 + h) * PIECES;
+  };
+
+  const Factors f = HALF && blockIdx.y ? pr.f[1] : pr.f[0];
 
   // each XCD takes one run of the whole tiles of the matrices there are to do,
   // and one of the shares (32 bits: divisions by 64 cost as much as a step)
@@ -1248,7 +1278,6 @@ __global__ __launch_bounds__(256, 2) void k_product(
     steps = share + (part < more);
   }
 
-  const Factors f = HALF && blockIdx.y ? pr.f[1] : pr.f[0];
   const _Float16* src[2] = {
       f.a.p + b * f.a.batch + (int64_t)bi * NT * f.a.pitch + first * 32,
       f.b.p + b * f.b.batch + (int64_t)bj * NT * f.b.pitch + first * 32};
@@ -1271,8 +1300,8 @@ __global__ __launch_bounds__(256, 2) void k_product(
           __builtin_amdgcn_global_load_lds(
               (const __attribute__((address_space(1))) void*)(
                   src[o] + h * plane[o] + from[o][l] + step * 32),
-              (__attribute__((address_space(3))) void*)&lds[buffer][o][h]
-                  [(l * 4 + wave) * WAVE],
+              (__attribute__((address_space(3))) void*)(
+                  stage(buffer, o, h) + (l * 4 + wave) * WAVE),
               16, 0, 0);
   };
 
@@ -1282,6 +1311,10 @@ __global__ __launch_bounds__(256, 2) void k_product(
 #pragma unroll
     for (int j = 0; j < W; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
 
+  // Small tiles have the registers to bring in POLY's a before the loop: the
+  // ending of a block, 1.2 us of a product's 7 at 200 x 300, took 2.2 with it.
+  Old<NT> old;
+  if (E == POLY && NT == 64 && !shared) old.load(f.a, b, bi, bj);
 #pragma unroll
   for (int p = 0; p < BUFFERS - 1; ++p)
     if (p < steps) fetch(p, p);
@@ -1301,8 +1334,8 @@ __global__ __launch_bounds__(256, 2) void k_product(
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int ra = wi + t * 16 + lane % 16, rb = wj + t * 16 + lane % 16;
-        av[t][h] = lds[buffer][0][h][ra * 4 + (lane / 16 ^ (ra / 2 % 4))];
-        bv[t][h] = lds[buffer][1][h][rb * 4 + (lane / 16 ^ (rb / 2 % 4))];
+        av[t][h] = stage(buffer, 0, h)[ra * 4 + (lane / 16 ^ (ra / 2 % 4))];
+        bv[t][h] = stage(buffer, 1, h)[rb * 4 + (lane / 16 ^ (rb / 2 % 4))];
       }
     if (step + BUFFERS - 1 < steps)
       fetch(step + BUFFERS - 1,
@@ -1329,7 +1362,8 @@ __global__ __launch_bounds__(256, 2) void k_product(
         ((f32x4*)parts)[(i * W + j) * 256 + threadIdx.x] = acc[i][j];
     return;
   }
-  end_product<NT, E, T>(pr, f, b, bi, bj, acc, (_Float16*)lds);
+  if (E == POLY && NT != 64) old.load(f.a, b, bi, bj);
+  end_product<NT, E, T>(pr, f, b, bi, bj, acc, old, (_Float16*)lds);
 }
 
 // The tiles whose sum was shared out: its parts, in their order.
@@ -1337,7 +1371,7 @@ template <int NT, Ending E, typename T>
 __global__ __launch_bounds__(256) void k_join(
     Product pr, const int* __restrict__ active) {
   constexpr int W = NT / 32;
-  __shared__ half8 lds[NT * (NT + 8) / 8];
+  __shared__ half8 lds[end_size<NT>() / 8];
   const uint32_t tile = pr.whole + blockIdx.x;
   const uint32_t matrix = tile / (uint32_t)pr.tiles;
   if (active && matrix >= (uint32_t)active[0]) return;
@@ -1361,7 +1395,9 @@ __global__ __launch_bounds__(256) void k_join(
 #pragma unroll
       for (int j = 0; j < W; ++j)
         acc[i][j] += parts[((q * W + i) * W + j) * 256 + threadIdx.x];
-  end_product<NT, E, T>(pr, f, b, bi, bj, acc, (_Float16*)lds);
+  Old<NT> old;
+  if (E == POLY) old.load(f.a, b, bi, bj);
+  end_product<NT, E, T>(pr, f, b, bi, bj, acc, old, (_Float16*)lds);
 }
 
 // ---------------------------------------------------------------------
