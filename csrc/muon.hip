@@ -24,6 +24,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <tuple>
 #include <type_traits>
 #include <vector>
 
@@ -148,44 +149,150 @@ __device__ inline float4 next_momentum(const Momentum& q, float4 v, float4 g,
   return v;
 }
 
-// place[r] (see several()) for up to 256 rows of one matrix a block;
-// touched[b] = whether the push names a row of matrix b.
+// place[r] (see several()) for up to 256 rows of one matrix at a time, of a
+// sorted push; touched[b] = whether the push names a row of matrix b.
 __global__ __launch_bounds__(256) void k_places(
     int64_t* __restrict__ place, int* __restrict__ touched,
     const int64_t* __restrict__ rows, const int64_t* __restrict__ order,
-    int64_t n, int64_t m) {
+    int64_t n, int64_t m, int64_t windows) {
   __shared__ int64_t mine[256];
   __shared__ int64_t ends[2];
   const int64_t chunks = (m + 255) / 256;
-  const int64_t b = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-  const int64_t r0 = b * m + chunk * 256, count = min(m - chunk * 256,
-                                                      (int64_t)256);
-  mine[threadIdx.x] = -1;
-  if (threadIdx.x % WAVE == 0 && threadIdx.x < 2 * WAVE) {
-    // a push of every row has row r at place r
-    const int64_t x = threadIdx.x == 0 ? r0 : r0 + count;
-    const bool direct = x < n && rows[x] == x && (x == 0 || rows[x - 1] < x);
-    ends[threadIdx.x / WAVE] = direct ? x : lower_bound(rows, n, x);
-  }
-  __syncthreads();
-  const int64_t lo = ends[0], hi = ends[1];
-  if (chunk == 0 && threadIdx.x == 0) {
-    bool some = hi > lo;
-    if (!some) {
-      const int64_t at = lower_bound(rows, n, b * m);
-      some = at < n && rows[at] < (b + 1) * m;
+  for (int64_t w = blockIdx.x; w < windows; w += gridDim.x) {
+    const int64_t b = w / chunks, chunk = w % chunks;
+    const int64_t r0 = b * m + chunk * 256;
+    const int64_t count = min(m - chunk * 256, (int64_t)256);
+    mine[threadIdx.x] = -1;
+    if (threadIdx.x % WAVE == 0 && threadIdx.x < 2 * WAVE) {
+      // a push of every row has row r at place r
+      const int64_t x = threadIdx.x == 0 ? r0 : r0 + count;
+      const bool direct = x < n && rows[x] == x && (x == 0 || rows[x - 1] < x);
+      ends[threadIdx.x / WAVE] = direct ? x : lower_bound(rows, n, x);
     }
-    touched[b] = some;
+    __syncthreads();
+    const int64_t lo = ends[0], hi = ends[1];
+    if (chunk == 0 && threadIdx.x == 0) {
+      bool some = hi > lo;
+      if (!some) {
+        const int64_t at = lower_bound(rows, n, b * m);
+        some = at < n && rows[at] < (b + 1) * m;
+      }
+      touched[b] = some;
+    }
+    for (int64_t j = lo + threadIdx.x; j < hi; j += 256) {
+      const int64_t at = rows[j] - r0;  // within, unless rows are not sorted
+      if (at >= 0 && at < count && (j == lo || rows[j - 1] != rows[j]))
+        mine[at] = j + 1 < hi && rows[j + 1] == rows[j]
+                       ? several(j)
+                       : (order ? order[j] : j);
+    }
+    __syncthreads();
+    if (threadIdx.x < count) place[r0 + threadIdx.x] = mine[threadIdx.x];
+    __syncthreads();
   }
-  for (int64_t j = lo + threadIdx.x; j < hi; j += 256) {
-    const int64_t at = rows[j] - r0;  // within, unless rows are not sorted
-    if (at >= 0 && at < count && (j == lo || rows[j - 1] != rows[j]))
-      mine[at] = j + 1 < hi && rows[j + 1] == rows[j]
-                     ? several(j)
-                     : (order ? order[j] : j);
+}
+
+// The same of a push in any order, of up to SHORT places, with the rows and
+// their places in `sorted` and `order`.  A block reads the whole push and keeps
+// what names its 256 rows, each wave a quarter of the push, so that equal rows
+// stay in the order that they came in.  Rows outside the table are in nobody's
+// window; the sorted rows end with -1 then.
+constexpr int SHORT = 16384;
+
+__global__ __launch_bounds__(256) void k_places_any(
+    int64_t* __restrict__ place, int* __restrict__ touched,
+    int64_t* __restrict__ sorted, int64_t* __restrict__ order,
+    const int64_t* __restrict__ rows, int n, int64_t m, int64_t total) {
+  __shared__ uint32_t list[SHORT + 3];  // row in the window, place in the push
+  __shared__ int next[4][256];          // a row's: how many, then where to
+  __shared__ int only[256], ends[4][2], sums[4];
+  const int64_t chunks = (m + 255) / 256;
+  const int64_t b = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+  const int64_t r0 = b * m + chunk * 256;
+  const int count = min(m - chunk * 256, (int64_t)256);
+  const int lane = threadIdx.x % WAVE, wave = this_wave(), t = threadIdx.x;
+  const uint64_t under = (1ull << lane) - 1;
+  const int share = (n + 3) / 4, from = min(wave * share, n);
+  const int to = min(from + share, n);
+  uint32_t* mine = list + wave * share;
+  int held = 0, before = 0, here = 0;
+  for (int w = 0; w < 4; ++w) next[w][t] = 0;
+  __syncthreads();
+  for (int j0 = from; j0 < to; j0 += 4 * WAVE) {
+    int64_t r[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int j = j0 + q * WAVE + lane;
+      r[q] = j < to ? rows[j] : -1;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t at = r[q] - r0;
+      const bool in = at >= 0 && at < count;
+      const uint64_t votes = __ballot(in);
+      before += __popcll(__ballot(r[q] >= 0 && r[q] < r0));
+      here |= __ballot(r[q] >= b * m && r[q] < (b + 1) * m) != 0;
+      if (in) {
+        atomicAdd(&next[wave][at], 1);
+        mine[held + __popcll(votes & under)] =
+            (uint32_t)at << 16 | (j0 + q * WAVE + lane);
+      }
+      held += __popcll(votes);
+    }
+  }
+  if (lane == 0) {
+    ends[wave][0] = before;
+    ends[wave][1] = here;
   }
   __syncthreads();
-  if (threadIdx.x < count) place[r0 + threadIdx.x] = mine[threadIdx.x];
+  // where row t's run begins among the sorted ones, and each wave's share of it
+  int named = 0;
+  for (int w = 0; w < 4; ++w) named += next[w][t];
+  int run = named;
+#pragma unroll
+  for (int o = 1; o < WAVE; o *= 2) {
+    const int left = __shfl_up(run, o);
+    if (lane >= o) run += left;
+  }
+  if (lane == WAVE - 1) sums[wave] = run;
+  __syncthreads();
+  for (int w = 0; w < 4; ++w) run += ends[w][0] + (w < wave ? sums[w] : 0);
+  const int first = run - named;
+  for (int w = 0, at = first; w < 4; ++w) {
+    const int more = next[w][t];
+    next[w][t] = at;
+    at += more;
+  }
+  __syncthreads();
+  // 64 of a wave's at a time: a row's place moves on by those that name it
+  for (int e = 0; e < held; e += WAVE) {
+    const bool some = e + lane < held;
+    const uint32_t v = some ? mine[e + lane] : 0;
+    const int r = v >> 16, j = v & 0xffff;
+    uint64_t same = __ballot(some);
+#pragma unroll
+    for (int bit = 0; bit < 8; ++bit) {
+      const uint64_t set = __ballot(r >> bit & 1);
+      same &= r >> bit & 1 ? set : ~set;
+    }
+    const int at = next[wave][r];
+    __builtin_amdgcn_wave_barrier();
+    if (some) {
+      const int mine_at = at + __popcll(same & under);
+      sorted[mine_at] = r0 + r;
+      order[mine_at] = j;
+      only[r] = j;
+      if (!(same >> lane >> 1)) next[wave][r] = mine_at + 1;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  if (t < count)
+    place[r0 + t] = named > 1 ? several(first) : named ? only[t] : -1;
+  if (t == 255 && r0 + count == total && run < n) sorted[run] = -1;
+  if (t == 0 && chunk == 0)
+    touched[b] = ends[0][1] | ends[1][1] | ends[2][1] | ends[3][1];
 }
 
 // active[0] = how many of up to 32768 matrices are touched, then which.
@@ -1872,7 +1979,7 @@ at::Tensor orthogonalize(at::Tensor x, int64_t steps, double a, double b,
 }
 
 void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
-                c10::optional<at::Tensor> order, at::Tensor grads, double lr,
+                bool sorted_unique, at::Tensor grads, double lr,
                 double mu, bool nesterov, double weight_decay, int64_t steps,
                 int64_t matrix_rows, double a, double b, double c,
                 double eps) {
@@ -1889,10 +1996,6 @@ void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
                   grads.scalar_type() == at::kFloat && grads.dim() == 2 &&
                   grads.size(0) == n && grads.size(1) == dim,
               "grads must be float32, one row for each int64 of rows");
-  TORCH_CHECK(!order || (order->scalar_type() == at::kLong &&
-                         order->numel() == n && order->is_contiguous() &&
-                         order->device() == table.device()),
-              "order must be int64, one for each row");
   TORCH_CHECK(matrix_rows >= 1 && table.size(0) % matrix_rows == 0,
               "the table is not a whole number of matrices of ", matrix_rows,
               " rows");
@@ -1905,15 +2008,32 @@ void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
   auto touched = at::empty({batch}, table.options().dtype(at::kInt));
   auto u = at::empty_like(table);
   auto place = at::empty({total}, rows.options());
-  hipLaunchKernelGGL(k_places,
-                     dim3(batch * ((matrix_rows + 255) / 256)), dim3(256), 0,
-                     stream, place.data_ptr<int64_t>(),
-                     touched.data_ptr<int>(), rows.data_ptr<int64_t>(),
-                     order ? order->data_ptr<int64_t>() : nullptr, n,
-                     matrix_rows);
+  const int64_t windows = batch * ((matrix_rows + 255) / 256);
+  at::Tensor order;
+  int64_t* at_ = place.data_ptr<int64_t>();
+  // Blocks that each read the whole push, against a sort and k_places (the
+  // whole step): 5000 places and 16 windows 41 us, 78; 9000 and 48 417, 441;
+  // 16000 and 1 (all of them in it) 97, 153; 16000 and 1024 65, 85
+  if (!sorted_unique && n <= SHORT && windows <= 1024) {
+    const auto push = rows;
+    rows = at::empty_like(push);
+    order = at::empty_like(push);
+    hipLaunchKernelGGL(k_places_any, dim3(windows), dim3(256), 0, stream, at_,
+                       touched.data_ptr<int>(), rows.data_ptr<int64_t>(),
+                       order.data_ptr<int64_t>(), push.data_ptr<int64_t>(),
+                       (int)n, matrix_rows, total);
+  } else {
+    if (!sorted_unique)
+      std::tie(rows, order) = at::sort(rows, /*stable=*/true, 0, false);
+    hipLaunchKernelGGL(k_places, dim3(std::min<int64_t>(windows, 1 << 20)),
+                       dim3(256), 0, stream, at_, touched.data_ptr<int>(),
+                       rows.data_ptr<int64_t>(),
+                       order.defined() ? order.data_ptr<int64_t>() : nullptr,
+                       n, matrix_rows, windows);
+  }
   const Momentum q{u.data_ptr<float>(),       momentum.data_ptr<float>(),
                    grads.data_ptr<float>(),   rows.data_ptr<int64_t>(),
-                   order ? order->data_ptr<int64_t>() : nullptr,
+                   order.defined() ? order.data_ptr<int64_t>() : nullptr,
                    n,                         (float)mu,
                    nesterov};
   // one pass makes U and sums G where a block holds a row and a square of G

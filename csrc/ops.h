@@ -17,7 +17,7 @@ at::Tensor cache_read(at::Tensor cache, int64_t dim,
 at::Tensor orthogonalize(at::Tensor x, int64_t steps, double a, double b,
                          double c, double eps);
 void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
-                c10::optional<at::Tensor> order, at::Tensor grads, double lr,
+                bool sorted_unique, at::Tensor grads, double lr,
                 double mu, bool nesterov, double weight_decay, int64_t steps,
                 int64_t matrix_rows, double a, double b, double c,
                 double eps);

@@ -2354,9 +2354,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("orthogonalize", &orthogonalize, "Newton-Schulz orthogonalisation",
         py::arg("x"), py::arg("steps"), py::arg("a"), py::arg("b"),
         py::arg("c"), py::arg("eps"));
-  m.def("apply_muon", &apply_muon, "Muon step over a row-sorted push",
+  m.def("apply_muon", &apply_muon, "Muon step over a push of rows",
         py::arg("table"), py::arg("momentum"), py::arg("rows"),
-        py::arg("order"), py::arg("grads"), py::arg("lr"), py::arg("mu"),
+        py::arg("sorted_unique"), py::arg("grads"), py::arg("lr"),
+        py::arg("mu"),
         py::arg("nesterov"), py::arg("weight_decay"), py::arg("steps"),
         py::arg("matrix_rows"), py::arg("a"), py::arg("b"), py::arg("c"),
         py::arg("eps"));

@@ -330,14 +330,13 @@ def apply_muon(table: torch.Tensor, momentum: torch.Tensor,
     if not rows.numel() or not table.numel():
         return
     rows, grads = rows.long().contiguous(), grads.detach().contiguous()
-    order = None
-    if not sorted_unique:
-        rows, order = torch.sort(rows, stable=True)
     args = (lr, mu, nesterov, weight_decay, int(steps), m)
     if _cuda(table):
-        hip.ext().apply_muon(table, momentum, rows, order, grads,
+        hip.ext().apply_muon(table, momentum, rows, bool(sorted_unique), grads,
                              *args, a, b, c, float(eps))
         return
-    reference.apply_muon(table, momentum, rows,
-                         grads if order is None else grads[order],
-                         *args, (a, b, c), float(eps))
+    if not sorted_unique:
+        rows, order = torch.sort(rows, stable=True)
+        grads = grads[order]
+    reference.apply_muon(table, momentum, rows, grads, *args, (a, b, c),
+                         float(eps))

@@ -16,6 +16,7 @@ once: half its eps relative to the result.
 """
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -364,6 +365,54 @@ def test_apply_muon_orders_and_index_types(device):
     assert torch.equal(five[0], table) and int(five[1].abs().sum()) == 0
     six = step(rows[:0], grads[:0])
     assert torch.equal(six[0], table)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("matrices_,m,pushed,skew", [
+    (1, 1000, 5000, 0.0), (3, 700, 16384, 0.6), (2, 300, 16385, 0.3),
+    (2, 256, 513, 0.0), (2, 257, 3, 0.0), (1, 5, 16384, 0.0),
+    (1024, 3, 700, 0.5), (1025, 3, 700, 0.5)])
+def test_unsorted_pushes_sum_in_their_order(device, matrices_, m, pushed,
+                                            skew):
+    """M is mu M + g to the bit, with g summed in f32 in the push's order;
+    pushes and tables on both sides of where they are sorted first."""
+    g = torch.Generator().manual_seed(pushed + m)
+    R, n, mu = matrices_ * m, 5, 0.5
+    rows = torch.randint(-3, R + 3, (pushed,), generator=g)
+    rows[torch.rand(pushed, generator=g) < skew] = R - 1
+    grads = torch.randn(pushed, n, generator=g)
+    mo = torch.randn(R, n, generator=g)
+    total = np.zeros((R, n), dtype=np.float32)
+    inside = (rows >= 0) & (rows < R)
+    np.add.at(total, rows[inside].numpy(), grads[inside].numpy())
+    named = torch.zeros(matrices_, dtype=torch.bool)
+    named[rows[inside] // m] = True
+    want = torch.where(named.repeat_interleave(m)[:, None],
+                       mu * mo + torch.from_numpy(total), mo)
+    t, v = torch.zeros(R, n, device=device), mo.to(device)
+    ops.apply_muon(t, v, rows.to(device), grads.to(device), 0.1, mu=mu,
+                   matrix_rows=m)
+    assert torch.equal(v.cpu(), want)  # a product by 1/2 is exact
+    assert torch.equal(t.cpu().view(matrices_, -1).any(1), named)
+
+
+@pytest.mark.gpu
+def test_more_matrices_than_a_grid():
+    """1,100,000 matrices of one value: each is its own sign, five steps on."""
+    R = 1100000
+    u, w = torch.randn(R, 1), torch.randn(R, 1)
+    t, v = w.cuda(), torch.zeros(R, 1, device="cuda")
+    ops.apply_muon(t, v, torch.arange(R).cuda(), u.cuda(), 0.1, mu=0.0,
+                   matrix_rows=1, sorted_unique=True)
+    x = u.double() / (u.double().abs() + 1e-7)
+    a, b, c = ops.MUON_COEFFS
+    for _ in range(5):
+        x = x * (a + b * x ** 2 + c * x ** 4)
+    # P and U in two planes each (2^-22), their lows' product left out (2^-22),
+    # f32 sums; then the weights' own roundings
+    limit = 0.1 * 8 * 2.0 ** -22 * x.abs() + 2 * U * (w.abs() + 0.2).double()
+    assert bool(((t.cpu().double() - (w.double() - 0.1 * x)).abs()
+                 <= limit).all())
 
 
 @pytest.mark.gpu
