@@ -1324,20 +1324,23 @@ __device__ inline void end_product(const Product& pr, const Factors& f,
   }
 }
 
-// A block an NT x NT tile of D (or its share of the sum), four waves a quarter
-// each, 32 places of K at a time: while the matrix instructions work on one of
-// the LDS buffers, the places that follow go from memory to the others without
-// a stop in registers.  A row of a buffer is four 16-byte pieces; piece c of
-// row r lies at c ^ (r / 2 % 4), so that eight lanes that read one piece of
-// eight rows hit different banks.  Three products of 16 cycles for each pair of
-// 16 x 16 x 32 operands.
-template <int NT, int BUFFERS, Ending E, typename T>
+// A block an NT x NT tile of D (or its share of the sum): while the matrix
+// instructions work on one of the LDS buffers, the places that follow go from
+// memory to the others without a stop in registers.  KH = 1: a wave takes a
+// quarter of the tile, 32 places at a time.  KH = 2: 64 places at a time, whole
+// lines; a wave takes half of the tile's columns and half of the places, which
+// are a quarter fewer LDS reads, and then two waves add their halves.  A row of
+// a buffer is PER 16-byte pieces, turned so that eight lanes that read one
+// piece of eight rows hit different banks.  Three products of 16 cycles for
+// each pair of 16 x 16 x 32 operands.
+template <int NT, int KH, int BUFFERS, Ending E, typename T>
 __global__ __launch_bounds__(256, 2) void k_product(
     Product pr, const int* __restrict__ active) {
   constexpr bool HALF = E == GRAM || E == POLY;
-  constexpr int W = NT / 32;           // 16-tiles a wave on each side
-  constexpr int LOADS = NT / 64;       // pieces a thread, operand and plane
-  constexpr int PIECES = NT * 4;       // of an operand's plane
+  constexpr int PLACES = 32 * KH, PER = PLACES / 8;
+  constexpr int W = NT / 32, R = W * KH;  // a wave's 16-tiles: R rows of W
+  constexpr int PIECES = NT * PER;        // of an operand's plane
+  constexpr int LOADS = PIECES / 256;     // a thread's
   constexpr int STAGE = BUFFERS * 4 * PIECES, LAST = end_size<NT>() / 8;
   __shared__ half8 lds[STAGE > LAST ? STAGE : LAST];
   auto stage = [&](int buffer, int operand, int h) {
@@ -1377,8 +1380,10 @@ __global__ __launch_bounds__(256, 2) void k_product(
   tile_of<HALF>(tile - matrix * pr.tiles, pr.ns, pr.nl, &bi, &bj);
 
   const int lane = threadIdx.x % WAVE, wave = this_wave();
-  const int wi = wave / 2 * (NT / 2), wj = wave % 2 * (NT / 2);
-  int first = 0, steps = pr.k / 32;
+  const int kh = KH == 2 ? wave / 2 : 0;
+  const int wi = KH == 2 ? 0 : wave / 2 * (NT / 2), wj = wave % 2 * (NT / 2);
+  auto turned = [](int r, int c) { return c ^ (r * PER / 8 % PER); };
+  int first = 0, steps = (pr.k + PLACES - 1) / PLACES;
   if (shared) {
     const uint32_t share = steps / splits, more = steps - share * splits;
     first = part * share + min(part, more);
@@ -1386,14 +1391,14 @@ __global__ __launch_bounds__(256, 2) void k_product(
   }
 
   const _Float16* src[2] = {
-      f.a.p + b * f.a.batch + (int64_t)bi * NT * f.a.pitch + first * 32,
-      f.b.p + b * f.b.batch + (int64_t)bj * NT * f.b.pitch + first * 32};
+      f.a.p + b * f.a.batch + (int64_t)bi * NT * f.a.pitch + first * PLACES,
+      f.b.p + b * f.b.batch + (int64_t)bj * NT * f.b.pitch + first * PLACES};
   const int64_t plane[2] = {f.a.plane, f.b.plane};
   int64_t from[2][LOADS];
 #pragma unroll
   for (int l = 0; l < LOADS; ++l) {
-    const int e = (l * 4 + wave) * WAVE + lane, r = e / 4;
-    const int c = (e % 4 ^ (r / 2 % 4)) * 8;
+    const int e = (l * 4 + wave) * WAVE + lane, r = e / PER;
+    const int c = turned(r, e % PER) * 8;
     from[0][l] = r * f.a.pitch + c;
     from[1][l] = r * f.b.pitch + c;
   }
@@ -1406,15 +1411,15 @@ __global__ __launch_bounds__(256, 2) void k_product(
         for (int l = 0; l < LOADS; ++l)
           __builtin_amdgcn_global_load_lds(
               (const __attribute__((address_space(1))) void*)(
-                  src[o] + h * plane[o] + from[o][l] + step * 32),
+                  src[o] + h * plane[o] + from[o][l] + step * PLACES),
               (__attribute__((address_space(3))) void*)(
                   stage(buffer, o, h) + (l * 4 + wave) * WAVE),
               16, 0, 0);
   };
 
-  f32x4 acc[W][W];
+  f32x4 acc[R][W];
 #pragma unroll
-  for (int i = 0; i < W; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
     for (int j = 0; j < W; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
 
@@ -1435,20 +1440,22 @@ __global__ __launch_bounds__(256, 2) void k_product(
                    :: "n"((BUFFERS - 2) * 4 * LOADS) : "memory");
     else
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    half8 av[W][2], bv[W][2];
+    half8 av[R][2], bv[W][2];
 #pragma unroll
-    for (int t = 0; t < W; ++t)
+    for (int t = 0; t < R; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int ra = wi + t * 16 + lane % 16, rb = wj + t * 16 + lane % 16;
-        av[t][h] = stage(buffer, 0, h)[ra * 4 + (lane / 16 ^ (ra / 2 % 4))];
-        bv[t][h] = stage(buffer, 1, h)[rb * 4 + (lane / 16 ^ (rb / 2 % 4))];
+        const int c = kh * 4 + lane / 16;
+        av[t][h] = stage(buffer, 0, h)[ra * PER + turned(ra, c)];
+        if (t < W)
+          bv[t % W][h] = stage(buffer, 1, h)[rb * PER + turned(rb, c)];
       }
     if (step + BUFFERS - 1 < steps)
       fetch(step + BUFFERS - 1,
             buffer ? buffer - 1 : BUFFERS - 1);
 #pragma unroll
-    for (int i = 0; i < W; ++i)
+    for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
@@ -1461,16 +1468,42 @@ __global__ __launch_bounds__(256, 2) void k_product(
     buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
   }
 
+  // a wave keeps the quarter of the tile that is its number's
+  f32x4 sum[W][W];
+  if (KH == 2) {
+    f32x4* sent = (f32x4*)lds;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        sent[(wave * W + i) * W * WAVE + j * WAVE + lane] =
+            kh ? acc[i][j] : acc[(W + i) % R][j];
+        sum[i][j] = kh ? acc[(W + i) % R][j] : acc[i][j];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        sum[i][j] += sent[((wave ^ 2) * W + i) * W * WAVE + j * WAVE + lane];
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+      for (int j = 0; j < W; ++j) sum[i][j] = acc[i][j];
+  }
+
   if (shared) {
 #pragma unroll
     for (int i = 0; i < W; ++i)
 #pragma unroll
       for (int j = 0; j < W; ++j)
-        ((f32x4*)parts)[(i * W + j) * 256 + threadIdx.x] = acc[i][j];
+        ((f32x4*)parts)[(i * W + j) * 256 + threadIdx.x] = sum[i][j];
     return;
   }
   if (E == POLY && NT != 64) old.load(f.a, b, bi, bj);
-  end_product<NT, E, T>(pr, f, b, bi, bj, acc, old, (_Float16*)lds);
+  end_product<NT, E, T>(pr, f, b, bi, bj, sum, old, (_Float16*)lds);
 }
 
 // The tiles whose sum was shared out: its parts, in their order.
@@ -1732,8 +1765,14 @@ void run_product(const Chain& c, Product pr, const Cut& cut, int jobs = 1) {
       hipLaunchKernelGGL(join, dim3(rest, jobs), dim3(256), 0, c.stream, pr,
                          c.active);
   };
-  if (cut.tile == 128) go(k_product<128, 2, E, T>, k_join<128, E, T>);
-  else go(k_product<64, 4, E, T>, k_join<64, E, T>);
+  // Of small tiles, two blocks on a CU wait for LDS and one for its loads: it
+  // needs them further ahead than buffers of 64 places reach.  Measured, KH = 2
+  // against 1: 12 x 512 x 1024 340 us, 362; 1500 x 2048 477, 544; 3 x 300 x
+  // 1001 178, 159; 200 x 300 116, 104
+  const int64_t blocks = (cut.whole + rest * cut.splits) * jobs;
+  if (cut.tile == 128) go(k_product<128, 1, 2, E, T>, k_join<128, E, T>);
+  else if (blocks > 256) go(k_product<64, 2, 2, E, T>, k_join<64, E, T>);
+  else go(k_product<64, 1, 4, E, T>, k_join<64, E, T>);
 }
 
 // How many steps in a row are taken on the Gram matrix before P is applied to
