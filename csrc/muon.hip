@@ -1123,7 +1123,8 @@ __global__ __launch_bounds__(256) void k_sumsq(
 }
 
 // The planes of X as it lies in memory (m x n) and transposed, 64 x 64 values
-// a block, zeros around them.
+// a block, zeros around them.  The values are on their way while the norm is
+// summed, and go out four at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void k_planes(
     Planes nat, Planes trn, const T* __restrict__ u,
@@ -1133,26 +1134,47 @@ __global__ __launch_bounds__(256) void k_planes(
   __shared__ double sums[4];
   const int64_t b = blockIdx.z;
   if (touched && !touched[b]) return;
+  const int64_t wide = nat.pitch / 64;
+  const int64_t r0 = blockIdx.x / wide * 64, c0 = blockIdx.x % wide * 64;
+  float4 v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t r = r0 + threadIdx.x / 16 + k * 16;
+    const int64_t c = c0 + threadIdx.x % 16 * 4;
+    v[k] = load_quad(u + (b * m + r) * n + c, r < m ? n - c : 0);
+  }
   double t = 0;
   for (int k = threadIdx.x; k < parts; k += 256) t += part[b * parts + k];
   const double2 f = norm_factors(block_sum(t, sums), eps);
   const float2 sc = make_float2((float)f.x, (float)f.y);
-  const int64_t wide = nat.pitch / 64;
-  const int64_t r0 = blockIdx.x / wide * 64, c0 = blockIdx.x % wide * 64;
-  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-    int r = e / 64, c = e % 64;
-    float v = 0.0f;
-    if (r0 + r < m && c0 + c < n)
-      v = to_f32(u[(b * m + r0 + r) * n + c0 + c]) * sc.x * sc.y * UP;
-    lds[r][c] = v;
-    _Float16* to = nat.p + b * nat.batch + (r0 + r) * nat.pitch + c0 + c;
-    split(v, to[0], to[nat.plane]);
+  auto put = [](const Planes& to, int64_t at, const float (&x)[4]) {
+    half4 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      _Float16 h, l;
+      split(x[i], h, l);
+      hi[i] = h;
+      lo[i] = l;
+    }
+    *(half4*)(to.p + at) = hi;
+    *(half4*)(to.p + at + to.plane) = lo;
+  };
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int r = threadIdx.x / 16 + k * 16, c = threadIdx.x % 16 * 4;
+    const float x[4] = {v[k].x * sc.x * sc.y * UP, v[k].y * sc.x * sc.y * UP,
+                        v[k].z * sc.x * sc.y * UP, v[k].w * sc.x * sc.y * UP};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lds[r][c + i] = x[i];
+    put(nat, b * nat.batch + (r0 + r) * nat.pitch + c0 + c, x);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-    int c = e / 64, r = e % 64;
-    _Float16* to = trn.p + b * trn.batch + (c0 + c) * trn.pitch + r0 + r;
-    split(lds[r][c], to[0], to[trn.plane]);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int c = threadIdx.x / 16 + k * 16, r = threadIdx.x % 16 * 4;
+    const float x[4] = {lds[r][c], lds[r + 1][c], lds[r + 2][c],
+                        lds[r + 3][c]};
+    put(trn, b * trn.batch + (c0 + c) * trn.pitch + r0 + r, x);
   }
 }
 
