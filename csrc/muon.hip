@@ -1578,6 +1578,7 @@ struct Chain {
   Result res;
   at::TensorOptions options;
   hipStream_t stream;
+  bool thin = false;
   // Muon: U comes from these; with `fused` the pass that sums G makes it,
   // without it is there
   bool fused = false;
@@ -1585,14 +1586,20 @@ struct Chain {
   const int64_t* place = nullptr;
 };
 
-bool is_thin(int64_t batch, int64_t m, int64_t n) {
+// Measured, thin against wide.  f32: 1 x 128 x 512 82 us, 98; 1 x 200 x 600
+// 104, 118; 1 x 256 x 512 115, 111; 1 x 320 x 1280 137, 162; of many matrices
+// the small products take longer: 4 x 200 x 800 147, 130; 16 x 128 x 1024 158,
+// 141; 8 x 200 x 3200 225, 246; 16 x 128 x 2048 164, 193.  bfloat16, whose wide
+// chain takes steps on G too: 1 x 200 x 600 108, 116; 2 x 200 x 1600 133, 137;
+// 1 x 256 x 1024 133, 123; 1 x 256 x 4096 134, 140; 1 x 320 x 5120 172, 158;
+// 2 x 256 x 4096 168, 146; 16 x 200 x 6400 553, 402
+bool is_thin(at::ScalarType type, int64_t batch, int64_t m, int64_t n) {
   const int64_t s = std::min(m, n), long_ = std::max(m, n);
-  // measured, thin against wide: 1 x 128 x 2048 95 us, 139; 4 x 128 x 512 107,
-  // 109; 16 x 128 x 512 163, 110; 256 x 4096 177, 178; 320 x 5000 249, 224
-  return s <= NARROW || (s <= THIN_MAX && long_ >= 32 * s) ||
-         (s <= SUPER && long_ >= 4 * s && batch * s <= 4 * SUPER);
+  if (s <= NARROW) return true;
+  if (type == at::kBFloat16)
+    return s <= 256 && batch * s <= 448 && long_ >= (s <= 224 ? 3 : 8) * s;
+  return s <= THIN_MAX && long_ >= (batch * s <= 512 ? 3 : 16) * s;
 }
-
 
 // How far P's values can reach: its value at singular values from 0 to 1.
 struct Reach {
@@ -1955,7 +1962,7 @@ int thin_round(const Coeffs& k, int steps) {
 
 template <typename T>
 void run(const Chain& c) {
-  if (!is_thin(c.batch, c.m, c.n)) {
+  if (!c.thin) {
     run_wide<T>(c);
     return;
   }
@@ -1986,9 +1993,11 @@ void run(const Chain& c) {
 }
 
 void dispatch(const Chain& whole) {
-  // grids hold 65535 matrices
+  // grids hold 65535 matrices; all of them take the same route
+  const bool thin = is_thin(whole.type, whole.batch, whole.m, whole.n);
   for (int64_t b = 0; b < whole.batch; b += 32768) {
     Chain c = whole;
+    c.thin = thin;
     const int64_t size = c.m * c.n * b;
     c.batch = std::min<int64_t>(32768, whole.batch - b);
     c.u = (const char*)c.u + size * c10::elementSize(c.type);
@@ -1997,7 +2006,7 @@ void dispatch(const Chain& whole) {
     at::Tensor active;
     if (c.touched) {
       c.touched += b;
-      if (!is_thin(c.batch, c.m, c.n)) {
+      if (!c.thin) {
         active = at::empty({c.batch + 1}, c.options.dtype(at::kInt));
         c.active = active.data_ptr<int>();
         hipLaunchKernelGGL(k_active, dim3(1), dim3(1024), 0, c.stream,
@@ -2030,7 +2039,7 @@ at::Tensor orthogonalize(at::Tensor x, int64_t steps, double a, double b,
   c10::DeviceGuard guard(x.device());
   auto out = at::empty_like(x);
   if (!x.numel()) return out;
-  if (type != at::kFloat && is_thin(x.size(0), x.size(1), x.size(2)) &&
+  if (type != at::kFloat && is_thin(type, x.size(0), x.size(1), x.size(2)) &&
       thin_round({a, b, c}, steps) < steps)
     return orthogonalize(x.to(at::kFloat), steps, a, b, c, eps).to(type);
   dispatch(Chain{x.data_ptr(), type, x.size(0), x.size(1), x.size(2), nullptr,
@@ -2098,7 +2107,7 @@ void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
                    n,                         (float)mu,
                    nesterov};
   // one pass makes U and sums G where a block holds a row and a square of G
-  const bool fused = is_thin(batch, matrix_rows, dim) && dim > NARROW &&
+  const bool fused = is_thin(at::kFloat, batch, matrix_rows, dim) && dim > NARROW &&
                      dim <= SUPER && matrix_rows >= dim && batch <= 32768;
   if (!fused) {
     int group = 1;

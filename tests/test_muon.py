@@ -105,6 +105,30 @@ def test_orthogonalize_large(b, m, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16,
+                                   torch.float16])
+@pytest.mark.parametrize("b,m,n", [
+    (1, 130, 390), (1, 390, 130), (1, 224, 672), (1, 225, 675), (1, 673, 224),
+    (1, 257, 800), (1, 320, 961), (1, 961, 320), (1, 256, 2048),
+    (3, 400, 129), (2, 225, 1800), (4, 3300, 200), (8, 70, 1121),
+    (9, 64, 66), (9, 65, 220)])
+def test_where_the_routes_meet(b, m, n, dtype):
+    x = matrices("decay", b, m, n, 15).to(dtype)
+    got = ops.orthogonalize(x.cuda())
+    for k in range(b):
+        check(got[k], x[k])
+
+
+@pytest.mark.gpu
+def test_more_matrices_than_a_launch():
+    """The last one, in a launch of its own, takes the others' route."""
+    x = torch.randn(32769, 65, 200, device="cuda", dtype=torch.float16)
+    got = ops.orthogonalize(x, steps=9)
+    for k in (0, 20000, 32767, 32768):
+        check(got[k], x[k].cpu(), steps=9)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("steps", [6, 7, 12, 13, 20, 100])
 @pytest.mark.parametrize("m,n", [(24, 40), (2000, 40), (600, 128),
@@ -299,7 +323,8 @@ def muon_by_hand(table, momentum, rows, grads, m, lr, mu, nesterov, wd):
 @pytest.mark.parametrize("matrices_,m,n,push", [
     (1, 40, 16, "all"), (1, 300, 8, "some"), (3, 20, 50, "repeats"),
     (4, 100, 120, "repeats"), (2, 150, 70, "all"), (5, 64, 64, "some"),
-    (3, 1, 9, "all"), (1, 1, 1, "repeats"), (2, 70, 1, "some")])
+    (3, 1, 9, "all"), (1, 1, 1, "repeats"), (2, 70, 1, "some"),
+    (2, 700, 200, "repeats"), (1, 200, 700, "some")])
 def test_apply_muon(device, nesterov, matrices_, m, n, push):
     g = torch.Generator().manual_seed(m + n)
     R = matrices_ * m
