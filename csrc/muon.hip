@@ -2075,16 +2075,26 @@ void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
   const int64_t total = table.size(0);
   c10::DeviceGuard guard(table.device());
   hipStream_t stream = at::hip::getCurrentHIPStream().stream();
+  // Blocks that each read the whole push, against a sort and k_places (the
+  // whole step): 5000 places and 16 windows 41 us, 78; 9000 and 48 417, 441;
+  // 16000 and 1 (all of them in it) 97, 153; 16000 and 1024 65, 85.  A sort
+  // clears memory in ways that a graph does not repeat: none is captured.
+  const int64_t windows = batch * ((matrix_rows + 255) / 256);
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  TORCH_CHECK(hipStreamIsCapturing(stream, &capture) == hipSuccess,
+              "the stream cannot be asked whether it is captured");
+  const bool captured = capture != hipStreamCaptureStatusNone;
+  const bool any = !sorted_unique && n <= SHORT &&
+                   (windows <= 1024 || (captured && windows <= 1 << 20));
+  TORCH_CHECK(sorted_unique || any || !captured, "a push of more than ", SHORT,
+              " rows in any order, or into more than ", 1 << 20,
+              " matrices, cannot be captured");
   auto touched = at::empty({batch}, table.options().dtype(at::kInt));
   auto u = at::empty_like(table);
   auto place = at::empty({total}, rows.options());
-  const int64_t windows = batch * ((matrix_rows + 255) / 256);
   at::Tensor order;
   int64_t* at_ = place.data_ptr<int64_t>();
-  // Blocks that each read the whole push, against a sort and k_places (the
-  // whole step): 5000 places and 16 windows 41 us, 78; 9000 and 48 417, 441;
-  // 16000 and 1 (all of them in it) 97, 153; 16000 and 1024 65, 85
-  if (!sorted_unique && n <= SHORT && windows <= 1024) {
+  if (any) {
     const auto push = rows;
     rows = at::empty_like(push);
     order = at::empty_like(push);

@@ -301,7 +301,8 @@ def apply_muon(table: torch.Tensor, momentum: torch.Tensor,
     with O as :func:`orthogonalize`.  The other matrices keep W and M.  Rows
     outside the table are left out.  Repeated rows are summed in the order
     that they come in.  ``sorted_unique``: the caller guarantees ``rows``
-    ascending with no duplicates, so the pre-sort is skipped."""
+    ascending with no duplicates, so the pre-sort is skipped.  Of other
+    pushes, those of up to 16384 rows can be captured into a graph."""
     a, b, c = _check_chain("apply_muon", steps, coeffs, eps)
     if table.dim() != 2 or table.dtype != torch.float32 \
             or momentum.shape != table.shape \

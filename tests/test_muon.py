@@ -556,6 +556,48 @@ def test_side_stream_and_replayed_graphs(m, n):
         assert torch.equal(table, t) and torch.equal(mo, v)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("matrices_,m,pushed", [(1, 300, 500), (3, 300, 16384),
+                                                (1100, 2, 700)])
+def test_unsorted_pushes_in_a_graph(matrices_, m, pushed):
+    R, n = matrices_ * m, 6
+    table, mo = (torch.randn(R, n, device="cuda") for _ in range(2))
+    rows = torch.randint(-2, R + 2, (pushed,), device="cuda")
+    grads = torch.randn(pushed, n, device="cuda")
+    ops.apply_muon(table, mo, rows, grads, 0.1, matrix_rows=m)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.apply_muon(table, mo, rows, grads, 0.1, matrix_rows=m)
+    for k in range(4):
+        rows.copy_(torch.randint(-2, R + 2, (pushed,), device="cuda"))
+        grads.copy_(torch.randn(pushed, n, device="cuda"))
+        t, v = table.clone(), mo.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        ops.apply_muon(t, v, rows, grads, 0.1, matrix_rows=m)
+        assert torch.equal(table, t) and torch.equal(mo, v)
+
+
+@pytest.mark.gpu
+def test_a_push_that_needs_a_sort_is_not_captured():
+    table, mo = torch.ones(300, 6, device="cuda"), torch.zeros(
+        300, 6, device="cuda")
+    rows = torch.randint(0, 300, (16385,), device="cuda")
+    grads = torch.randn(16385, 6, device="cuda")
+    one = torch.zeros(8, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        one += 1  # the graph has a node
+        with pytest.raises(RuntimeError, match="captured"):
+            ops.apply_muon(table, mo, rows, grads, 0.1)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bool((one == 1).all()) and bool((table == 1).all())
+    ops.apply_muon(table, mo, rows, grads, 0.1)  # not captured: it steps
+    assert not bool((table == 1).any())
+
+
 # -- the server ------------------------------------------------------------
 
 class Regress(WorkerLogic):
