@@ -26,7 +26,7 @@ from __future__ import annotations
 
 import collections
 from abc import ABC, abstractmethod
-from typing import Any, Callable, Optional, TypeVar
+from typing import Any, Callable, List, Optional, Tuple, TypeVar
 
 import torch
 
@@ -147,6 +147,13 @@ class ServerLogic(ABC):
     def on_push_recv(self, ids: torch.Tensor, deltas: torch.Tensor,
                      ps: ParameterServer) -> None:
         """Apply a batch of delta updates."""
+
+    def on_pushes_recv(self, pushes: List[Tuple[torch.Tensor, torch.Tensor]],
+                       ps: ParameterServer) -> None:
+        """Apply all the pushes that reached the shard in one round: the
+        ``(ids, deltas)`` of every worker that sent some, in rank order."""
+        for ids, deltas in pushes:
+            self.on_push_recv(ids, deltas, ps)
 
     def close(self, ps: ParameterServer) -> None:  # noqa: B027
         """Called once when the job drains; typically dumps the shard."""

@@ -203,6 +203,15 @@ class PSEngine:
                 "pushes_unique=False, whose apply path pre-aggregates "
                 "duplicates)")
 
+        # A limited pull is answered in parts, and a worker that pushes per
+        # answer would have a matrix take a step for each part of its rows.
+        if (self._pull_limit is not None and
+                getattr(server_logic, "whole_steps", False)):
+            raise ValueError(
+                "a pull limit may split a matrix's rows over several rounds, "
+                "and a server with optimizer='muon' steps a matrix in every "
+                "round that pushes one of its rows: use no pull limit")
+
     # ------------------------------------------------------------------
     def run(self, data: Iterable[Any], max_rounds: Optional[int] = None
             ) -> Tuple[List[Any], List[Any]]:
@@ -336,10 +345,7 @@ class PSEngine:
         r_pull, r_push_ids, r_push_deltas = recv
 
         # 5. server role: pushes first (fresher answers), then pulls
-        for s in range(self.world):
-            ids, deltas = r_push_ids[s], r_push_deltas[s]
-            if ids is not None and ids.numel():
-                self.server_logic.on_push_recv(ids, deltas, self.ps)
+        self._serve_pushes(r_push_ids, r_push_deltas)
         for s in range(self.world):
             ids = r_pull[s]
             if ids is not None and ids.numel():
@@ -513,10 +519,7 @@ class PSEngine:
 
         # 5. server phase: pushes first (fresher answers), then pulls;
         # produced answers are stashed for the NEXT round's exchange
-        for s in range(self.world):
-            ids, deltas = r_push_ids[s], r_push_deltas[s]
-            if ids is not None and ids.numel():
-                self.server_logic.on_push_recv(ids, deltas, self.ps)
+        self._serve_pushes(r_push_ids, r_push_deltas)
         for s in range(self.world):
             ids = r_pull[s]
             if ids is not None and ids.numel():
@@ -655,10 +658,7 @@ class PSEngine:
 
         # 5. server phase: pushes first (fresher answers), then pulls;
         # produced answers ship in the NEXT round's exchange.
-        for s in range(self.world):
-            ids, deltas = r_push_ids[s], r_push_deltas[s]
-            if ids is not None and ids.numel():
-                self.server_logic.on_push_recv(ids, deltas, self.ps)
+        self._serve_pushes(r_push_ids, r_push_deltas)
         for s in range(self.world):
             ids = r_pull[s]
             if ids is not None and ids.numel():
@@ -670,6 +670,22 @@ class PSEngine:
 
         done = bool(ctrl[:, 1].all())
         return exhausted, done
+
+    # ------------------------------------------------------------------
+    def _serve_pushes(self, ids: List[Optional[torch.Tensor]],
+                      deltas: List[Optional[torch.Tensor]]) -> None:
+        """Hand the round's pushes, one of every source that sent some, to
+        the server logic in rank order."""
+        pushes = [(i, d) for i, d in zip(ids, deltas)
+                  if i is not None and i.numel()]
+        if not pushes:
+            return
+        joint = getattr(self.server_logic, "on_pushes_recv", None)
+        if joint is not None:
+            joint(pushes, self.ps)
+            return
+        for i, d in pushes:
+            self.server_logic.on_push_recv(i, d, self.ps)
 
     # ------------------------------------------------------------------
     def _to_device(self, recv):

@@ -11,11 +11,12 @@ of the id), updated by HIP scatter-apply kernels.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 
 from . import ops
+from .api import ServerLogic
 from .parallel.partitioner import Partitioner
 
 
@@ -31,10 +32,12 @@ class ShardedTable:
                   M = momentum*M + g; W = (1-lr*weight_decay)*W -
                   lr*sqrt(max(1, m/n))*O, O the orthogonalised g +
                   momentum*M (``nesterov``) or M (ops.apply_muon).  Every
-                  push batch is one step of the matrices that it names a
-                  row of.  A matrix has to lie on one shard: with several
-                  shards use a RangePartitioner whose blocks hold whole
-                  matrices.  M is checkpointed as the accumulator.
+                  ``apply`` is one step of the matrices that it names a
+                  row of; TableServerLogic makes one of all the pushes
+                  that a round brings, whose gradients are summed (those of
+                  another round are another step).  A matrix has to lie on one shard: with several shards use
+                  a RangePartitioner whose blocks hold whole matrices.  M
+                  is checkpointed as the accumulator.
     """
 
     def __init__(self, part: Partitioner, shard: int, dim: int,
@@ -187,7 +190,7 @@ class ShardedTable:
                                                  self.data.dtype))
 
 
-class TableServerLogic:
+class TableServerLogic(ServerLogic):
     """ServerLogic over a ShardedTable — the production default server.
 
     Semantics parity: ``SimplePSLogic(paramInit, paramUpdate)`` with
@@ -198,6 +201,9 @@ class TableServerLogic:
     #: answers every pull batch in full, in received order, same round —
     #: lets the engine elide answer ids from the feedback edge.
     answers_in_order = True
+
+    # the push at hand is that of several workers, whose ids repeat
+    _joined = False
 
     def __init__(self, table: ShardedTable, dump_on_close: bool = True,
                  pushes_unique: bool = False):
@@ -212,12 +218,35 @@ class TableServerLogic:
         self.dump_on_close = dump_on_close
         self.pushes_unique = pushes_unique
 
+    @property
+    def whole_steps(self) -> bool:
+        """Whether an apply is a step of all the rows of what it touches, and
+        not a sum that may come in parts (Muon: of whole matrices)."""
+        return getattr(self.table, "optimizer", None) == "muon"
+
     def on_pull_recv(self, ids: torch.Tensor, worker: int, ps) -> None:
         ps.answer_pull(ids, self.table.gather(ids), worker)
 
     def on_push_recv(self, ids: torch.Tensor, deltas: torch.Tensor,
                      ps) -> None:
-        self.table.apply(ids, deltas, unique=self.pushes_unique)
+        self.table.apply(ids, deltas,
+                         unique=self.pushes_unique and not self._joined)
+
+    def on_pushes_recv(self, pushes: List[Tuple[torch.Tensor, torch.Tensor]],
+                       ps) -> None:
+        """A round's pushes one after the other, or, where an apply is a
+        whole step, as one push: a step of each would move a matrix as often
+        as there are workers, however small their shares of the gradient
+        are."""
+        if len(pushes) == 1 or not self.whole_steps:
+            super().on_pushes_recv(pushes, ps)
+            return
+        self._joined = True
+        try:
+            self.on_push_recv(torch.cat([i for i, _ in pushes]),
+                              torch.cat([d for _, d in pushes]), ps)
+        finally:
+            self._joined = False
 
     def close(self, ps) -> None:
         if self.dump_on_close:
