@@ -355,11 +355,12 @@ struct Norm { float x, y; };
 
 // X = U / n with n = |U|_F + eps as (u x) y: the power of two x keeps y and
 // the products normal for values near the ends of f32's range.  NaN for a
-// matrix that is not finite.
+// matrix that is not finite; zeros stay zeros whatever eps, whose reciprocal
+// may be more than an f32 holds.
 // eps < 0: U is X already.
 __device__ inline double2 norm_factors(double sumsq, double eps) {
   if (!(sumsq < INFINITY)) return make_double2(1.0, NAN);
-  if (eps < 0) return make_double2(1.0, 1.0);
+  if (eps < 0 || sumsq == 0) return make_double2(1.0, 1.0);
   const double n = sqrt(sumsq) + eps;
   const double x = n > 0x1p60 ? 0x1p-60 : (n < 0x1p-60 ? 0x1p60 : 1.0);
   return make_double2(x, 1.0 / (n * x));
