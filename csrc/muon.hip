@@ -350,20 +350,33 @@ constexpr int SUPER = 128;     // a block's square of G
 constexpr int KC = 32;         // long-axis places a block stages at a time
 constexpr int PITCH = SUPER + 16;
 
-// X = ((u x) y), what the product that applies P needs of the norm.
-struct Norm { float x, y; };
+// X = (u x) y t, what the product that applies P needs of the norm.
+struct Norm { float x, y, t; };
 
-// X = U / n with n = |U|_F + eps as (u x) y: the power of two x keeps y and
-// the products normal for values near the ends of f32's range.  NaN for a
-// matrix that is not finite; zeros stay zeros whatever eps, whose reciprocal
-// may be more than an f32 holds.
+// X = U / n with n = |U|_F + eps as (u x) y 2^e, with (u x) y of a norm between
+// 1/4 and 1, so that f16 planes of it hold their bits also where U is small
+// beside eps; e is 0 from |U|_F = eps up.  The power of two x keeps y and the
+// products normal for values near the ends of f32's range.  NaN for a matrix
+// that is not finite; zeros stay zeros whatever eps, whose reciprocal may be
+// more than an f32 holds.
 // eps < 0: U is X already.
-__device__ inline double2 norm_factors(double sumsq, double eps) {
-  if (!(sumsq < INFINITY)) return make_double2(1.0, NAN);
-  if (eps < 0 || sumsq == 0) return make_double2(1.0, 1.0);
-  const double n = sqrt(sumsq) + eps;
-  const double x = n > 0x1p60 ? 0x1p-60 : (n < 0x1p-60 ? 0x1p60 : 1.0);
-  return make_double2(x, 1.0 / (n * x));
+struct Unit {
+  double x, y;
+  int e;
+  __device__ inline double all() const { return ldexp(x * y, e); }
+  __device__ inline Norm norm() const {
+    return Norm{(float)x, (float)y, (float)ldexp(1.0, e)};
+  }
+};
+
+__device__ inline Unit unit_of(double sumsq, double eps) {
+  if (!(sumsq < INFINITY)) return {1.0, NAN, 0};
+  if (sumsq == 0) return {1.0, 1.0, 0};
+  const double u = sqrt(sumsq), n = eps < 0 ? 1.0 : u + eps;
+  const int e = min(0, ilogb(u) - ilogb(n) + 1);
+  const double own = ldexp(n, e);  // |U|_F to 4 |U|_F (eps < 0: no more than 1)
+  const double x = own > 0x1p60 ? 0x1p-60 : (own < 0x1p-60 ? 0x1p60 : 1.0);
+  return {x, 1.0 / (own * x), e};
 }
 
 __device__ inline void split(float v, _Float16& hi, _Float16& lo) {
@@ -748,10 +761,9 @@ __global__ __launch_bounds__(256) void k_gram_sum(
   const int count = chunks * ((sp + SUPER - 1) / SUPER);
   double t = 0;
   for (int k = threadIdx.x; k < count; k += 256) t += traces[b * count + k];
-  const double2 f = norm_factors(block_sum(t, sums), eps);
-  const double nu = f.x * f.y;
-  if (blockIdx.x == 0 && threadIdx.x == 0)
-    norm[b] = Norm{(float)f.x, (float)f.y};
+  const Unit f = unit_of(block_sum(t, sums), eps);
+  const double nu = f.all();
+  if (blockIdx.x == 0 && threadIdx.x == 0) norm[b] = f.norm();
   // 16 values a block, 16 threads a value
   __shared__ double slices[16][17];
   const int64_t size = (int64_t)sp * sp;
@@ -883,9 +895,9 @@ __global__ __launch_bounds__(WAVES * WAVE) void k_chain(
     __syncthreads();
   }
   const double trace = threadIdx.x < SP ? g[threadIdx.x * (LP + 1)] : 0.0;
-  const double2 f = norm_factors(block_sum(trace, sums), eps);
-  const double nu = f.x * f.y;
-  if (threadIdx.x == 0) norm[b] = Norm{(float)f.x, (float)f.y};
+  const Unit f = unit_of(block_sum(trace, sums), eps);
+  const double nu = f.all();
+  if (threadIdx.x == 0) norm[b] = f.norm();
   for (int o = threadIdx.x; o < SP * LP; o += WAVES * WAVE)
     if (o % LP < SP) g[o] *= nu * nu;
   __syncthreads();
@@ -982,6 +994,7 @@ __global__ __launch_bounds__(WAVES * WAVE) void k_thin_apply(
   const int j0 = blockIdx.y * JT * 16;
   const Norm nm = norm[b];
   const float up = nm.y * UP;
+  auto result = [&](float v) { return v * down * nm.t; };
   const T* x = u + b * long_ * s;
   const _Float16* p = planes + (b * jp + j0) * (int64_t)kp;
   const int64_t plane = gridDim.z * (int64_t)jp * kp;
@@ -1076,17 +1089,17 @@ __global__ __launch_bounds__(WAVES * WAVE) void k_thin_apply(
 #pragma unroll
         for (int w = 0; w < RT; ++w)
           finish_quad<T>(res, mine + at(w) * s + j,
-                         make_float4(acc[t][w][0] * down, acc[t][w][1] * down,
-                                     acc[t][w][2] * down,
-                                     acc[t][w][3] * down),
+                         make_float4(result(acc[t][w][0]), result(acc[t][w][1]),
+                                     result(acc[t][w][2]),
+                                     result(acc[t][w][3])),
                          at(w) < long_ ? s - j : 0);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           finish_quad<T>(res, mine + (int64_t)(j + i) * long_ + r0,
-                         make_float4(acc[t][0][i] * down, acc[t][1][i] * down,
-                                     acc[t][2 % RT][i] * down,
-                                     acc[t][3 % RT][i] * down),
+                         make_float4(result(acc[t][0][i]), result(acc[t][1][i]),
+                                     result(acc[t][2 % RT][i]),
+                                     result(acc[t][3 % RT][i])),
                          j + i < s ? long_ - r0 : 0);
       }
     }
@@ -1124,11 +1137,11 @@ __global__ __launch_bounds__(256) void k_sumsq(
 }
 
 // The planes of X as it lies in memory (m x n) and transposed, 64 x 64 values
-// a block, zeros around them.  The values are on their way while the norm is
-// summed, and go out four at a time.
+// a block, zeros around them, as 2^-e X (see unit_of); e goes to `small`.  The
+// values are on their way while the norm is summed, and go out four at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void k_planes(
-    Planes nat, Planes trn, const T* __restrict__ u,
+    Planes nat, Planes trn, int* __restrict__ small, const T* __restrict__ u,
     const double* __restrict__ part, int parts,
     const int* __restrict__ touched, int64_t m, int64_t n, double eps) {
   __shared__ float lds[64][65];
@@ -1146,8 +1159,9 @@ __global__ __launch_bounds__(256) void k_planes(
   }
   double t = 0;
   for (int k = threadIdx.x; k < parts; k += 256) t += part[b * parts + k];
-  const double2 f = norm_factors(block_sum(t, sums), eps);
+  const Unit f = unit_of(block_sum(t, sums), eps);
   const float2 sc = make_float2((float)f.x, (float)f.y);
+  if (blockIdx.x == 0 && threadIdx.x == 0) small[b] = f.e;
   auto put = [](const Planes& to, int64_t at, const float (&x)[4]) {
     half4 hi, lo;
 #pragma unroll
@@ -1187,8 +1201,23 @@ struct Factors {
   float scale;
 };
 
+// Planes of X hold 2^-e X with e = min(0, small[b] + grown), where the steps so
+// far multiply by 2^grown at most: a matrix that is small beside eps (see
+// unit_of) keeps its bits while it grows.
+struct Exponents {
+  const int* small;
+  int grown;  // of the X that the product takes
+  int times;  // how often it takes X
+  int next;   // UPDATE: `grown` of the X that it makes
+
+  __device__ inline int of(int64_t b, int g) const {
+    return min(0, small[b] + g);
+  }
+};
+
 struct Product {
   Factors f[2];      // blockIdx.y says which
+  Exponents e;
   int k;             // a multiple of 32
   Planes dt;         // UPDATE: D transposed (GRAM, POLY: D is symmetric)
   float ca, cb, cc;  // POLY: a I + b a + c D
@@ -1278,6 +1307,11 @@ __device__ inline void end_product(const Product& pr, const Factors& f,
   constexpr int W = NT / 32;
   const int lane = threadIdx.x % WAVE, wave = this_wave();
   const int wi = wave / 2 * (NT / 2), wj = wave % 2 * (NT / 2);
+  // what D has to be multiplied by for the exponents of its X
+  float by = 1.0f;
+  if (E != POLY)
+    by = ldexpf(1.0f, pr.e.times * pr.e.of(b, pr.e.grown) -
+                          (E == UPDATE ? pr.e.of(b, pr.e.next) : 0));
   if (E == FINAL) {
 #pragma unroll
     for (int ti = 0; ti < W; ++ti)
@@ -1286,7 +1320,7 @@ __device__ inline void end_product(const Product& pr, const Factors& f,
         const int64_t i = (int64_t)bi * NT + wi + ti * 16 + lane / 16 * 4;
         const int64_t j = (int64_t)bj * NT + wj + tj * 16 + lane % 16;
         if (j >= pr.cols) continue;
-        const f32x4 v = acc[ti][tj] * f.scale;
+        const f32x4 v = acc[ti][tj] * f.scale * by;
         const int64_t base = b * pr.rows * pr.cols;
         if (pr.tall) {
           finish_quad<T>(pr.res, base + j * pr.rows + i,
@@ -1305,6 +1339,7 @@ __device__ inline void end_product(const Product& pr, const Factors& f,
   constexpr int ROW = NT + 8;
   const bool both = E == UPDATE || bi != bj;
   const Planes& t = E == UPDATE ? pr.dt : f.d;
+  const float scale = f.scale * by;
   __syncthreads();
 #pragma unroll
   for (int ti = 0; ti < W; ++ti)
@@ -1313,7 +1348,7 @@ __device__ inline void end_product(const Product& pr, const Factors& f,
       const int li = wi + ti * 16 + lane / 16 * 4;
       const int lj = wj + tj * 16 + lane % 16;
       const int64_t i = (int64_t)bi * NT + li, j = (int64_t)bj * NT + lj;
-      const f32x4 v = acc[ti][tj] * f.scale;
+      const f32x4 v = acc[ti][tj] * scale;
       half4 hi, lo;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -1631,6 +1666,18 @@ struct Reach {
   }
 };
 
+// By how many powers of two the first i steps multiply a value at most.
+std::vector<int> growth(const Coeffs& k, int steps) {
+  Reach reach;
+  std::vector<int> g{0};
+  double power = 0;
+  for (int i = 0; i < steps; ++i) {
+    power += std::log2(std::max(reach.step(k), 0x1p-20));
+    g.push_back((int)std::ceil(power));
+  }
+  return g;
+}
+
 template <typename T, bool TALL>
 void run_thin(const Chain& c) {
   const int s = std::min(c.m, c.n);
@@ -1659,7 +1706,7 @@ void run_thin(const Chain& c) {
   auto f64 = c.options.dtype(at::kDouble);
   auto part = at::empty({c.batch * chunks * size}, f64);
   auto pl = at::empty({2 * c.batch * jp * kp}, c.options.dtype(at::kHalf));
-  auto nm = at::empty({c.batch * 2}, c.options.dtype(at::kFloat));
+  auto nm = at::empty({c.batch * 3}, c.options.dtype(at::kFloat));
   _Float16* planes = (_Float16*)pl.data_ptr();
   Norm* norm = (Norm*)nm.data_ptr();
   double* parts = part.data_ptr<double>();
@@ -1842,12 +1889,13 @@ void run_wide(const Chain& c) {
   const int parts = (int)std::min<int64_t>(
       std::max<int64_t>(1, 1024 / c.batch), (c.m * c.n + 4095) / 4096);
   auto part = at::empty({c.batch * parts}, c.options.dtype(at::kDouble));
+  auto small = at::empty({c.batch}, c.options.dtype(at::kInt));
   hipLaunchKernelGGL(k_sumsq<T>, dim3(parts, c.batch), dim3(256), 0, c.stream,
                      part.data_ptr<double>(), (const T*)c.u, c.touched,
                      c.m * c.n);
   hipLaunchKernelGGL(k_planes<T>, dim3(np / 64 * (mp / 64), 1, c.batch),
-                     dim3(256), 0, c.stream, nat, trn, (const T*)c.u,
-                     part.data_ptr<double>(), parts, c.touched, c.m, c.n,
+                     dim3(256), 0, c.stream, nat, trn, small.data_ptr<int>(),
+                     (const T*)c.u, part.data_ptr<double>(), parts, c.touched, c.m, c.n,
                      c.eps);
   const int64_t long_ = std::max(c.m, c.n);
   const Cut gram = cut_of(s, s, true, c.batch, long_);
@@ -1859,6 +1907,8 @@ void run_wide(const Chain& c) {
                                   cut.tile);
   auto sums = at::empty({2 * shared}, c.options.dtype(at::kFloat));
   Product pr{};
+  pr.e.small = small.data_ptr<int>();
+  const std::vector<int> grown = growth(c.k, c.steps);
   pr.ca = (float)c.k.a;
   pr.cb = (float)c.k.b;
   pr.cc = (float)c.k.c;
@@ -1874,19 +1924,23 @@ void run_wide(const Chain& c) {
   auto again = [&] { return tall ? planes(mp, np) : planes(np, mp); };
   Planes g = square(), q = square(), xt2{};
 
-  auto new_gram = [&] {
+  auto new_gram = [&](int done) {
     pr.f[0] = {x, x, g, down};
     pr.k = kl;
+    pr.e.grown = grown[done];
+    pr.e.times = 2;
     run_product<GRAM, T>(c, pr, gram);
+    pr.e.times = 0;
     pr.k = ks;
   };
   auto new_poly = [&](Planes to) {
     pr.f[0] = {g, g, to, down};
     run_product<POLY, T>(c, pr, poly);
   };
-  // X <- (by / held) X, the last time as the result
-  auto apply = [&](Planes by, float held, bool last) {
-    if (last) {
+  // X <- (by / held) X, after `to` steps, the last time as the result
+  auto apply = [&](Planes by, float held, int to) {
+    pr.e.times = 1;
+    if (to == c.steps) {
       pr.f[0] = {by, xt, x, down * down / held};
       run_product<FINAL, T>(c, pr, full);
       return;
@@ -1894,6 +1948,7 @@ void run_wide(const Chain& c) {
     if (!xt2.p) xt2 = again();
     pr.f[0] = {by, xt, x, down / held};
     pr.dt = xt2;
+    pr.e.next = grown[to];
     run_product<UPDATE, T>(c, pr, full);
     std::swap(xt, xt2);
   };
@@ -1901,9 +1956,9 @@ void run_wide(const Chain& c) {
   const int row = steps_on_gram<T>(c, s, long_);
   if (row == 1) {
     for (int i = 0; i < c.steps; ++i) {
-      new_gram();
+      new_gram(i);
       new_poly(q);
-      apply(q, 1.0f, i + 1 == c.steps);
+      apply(q, 1.0f, i + 1);
     }
     return;
   }
@@ -1914,7 +1969,7 @@ void run_wide(const Chain& c) {
     const int todo = std::min(row, c.steps - done);
     float held = 1.0f;  // P's planes hold P times this
     reach.start();
-    new_gram();
+    new_gram(done);
     for (int i = 0; i < todo; ++i) {
       const bool last = i + 1 == todo;
       const Planes qi = i ? q : p;
@@ -1938,7 +1993,7 @@ void run_wide(const Chain& c) {
       }
     }
     done += todo;
-    apply(p, held, done == c.steps);
+    apply(p, held, done);
   }
 }
 
