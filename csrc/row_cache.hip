@@ -459,6 +459,8 @@ void cache_write(at::Tensor cache, at::Tensor values,
                     "cache_write: 2^31 rows or more in one write");
   TORCH_CHECK(!(values.requires_grad() && c10::GradMode::is_enabled()),
               "cache_write has no gradient: pass values.detach()");
+  TORCH_CHECK(!values._fw_grad(0).defined(),
+              "cache_write has no gradient: an operand carries a tangent");
   if (!n) return;
   c10::DeviceGuard guard(cache.device());
   hipStream_t stream = at::hip::getCurrentHIPStream().stream();

@@ -271,6 +271,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5,
     a, b, c = _check_chain("orthogonalize", steps, coeffs, eps)
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("orthogonalize has no gradient: pass x.detach()")
+    reference.check_no_tangent("orthogonalize", x)
     if not x.numel():
         return torch.empty(x.shape, dtype=x.dtype, device=x.device)
     batch = x.detach().reshape(-1, *x.shape[-2:]).contiguous()
@@ -324,6 +325,7 @@ def apply_muon(table: torch.Tensor, momentum: torch.Tensor,
                          f"{grads.dtype} of {tuple(grads.shape)}")
     if not table.device == momentum.device == rows.device == grads.device:
         raise ValueError("apply_muon: operands on several devices")
+    reference.check_no_tangent("apply_muon", table, momentum, grads)
     m = table.shape[0] if matrix_rows is None else int(matrix_rows)
     if table.shape[0] and (m < 1 or table.shape[0] % m):
         raise ValueError(f"apply_muon: a table of {table.shape[0]} rows is "

@@ -24,6 +24,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 # ---------------------------------------------------------------------------
 # Deterministic per-element hashing (splitmix64) — must bit-match the HIP
@@ -333,6 +334,15 @@ _FP8_TOP = 240 * 2.0 ** 120  # the next code up stands for 2^128
 _INT8_TOP = 2.6793883890187504e+36
 
 
+def check_no_tangent(name: str, *operands: torch.Tensor) -> None:
+    """Refuse operands of forward-mode differentiation, whose tangents would
+    be dropped."""
+    for t in operands:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no gradient: an operand carries "
+                               "a tangent")
+
+
 def _check_records(name: str, cache: torch.Tensor, dim: int,
                    slots: Optional[torch.Tensor], fmt: str) -> None:
     """What the HIP entry points refuse, refused alike."""
@@ -376,6 +386,7 @@ def cache_write(cache: torch.Tensor, values: torch.Tensor,
     if values.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("cache_write has no gradient: pass "
                            "values.detach()")
+    check_no_tangent("cache_write", values)
     if not values.shape[0]:
         return
     x = values.detach().float()
