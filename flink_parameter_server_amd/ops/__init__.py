@@ -193,7 +193,8 @@ def cache_write(cache: torch.Tensor, values: torch.Tensor,
 
     ``fmt="int8"``: scale = amax / 127, equal steps; ``"fp8"``: e4m3 under a
     power-of-two scale, a relative error of at most 2^-4 a value down to
-    2^-15 of the row's largest.  A row with an infinity or NaN reads back as
+    1 / 14336 of the row's largest (for rows whose largest is 2^-118 or
+    more; smaller ones have a scale of 2^-126).  A row with an infinity or NaN reads back as
     NaN throughout.  Slots outside the cache are padding and not written.
     Of several rows for one slot the last one is kept; ``unique=True``
     asserts that there are none (and saves the pass that finds out)."""

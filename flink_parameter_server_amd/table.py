@@ -35,9 +35,10 @@ class ShardedTable:
                   ``apply`` is one step of the matrices that it names a
                   row of; TableServerLogic makes one of all the pushes
                   that a round brings, whose gradients are summed (those of
-                  another round are another step).  A matrix has to lie on one shard: with several shards use
-                  a RangePartitioner whose blocks hold whole matrices.  M
-                  is checkpointed as the accumulator.
+                  another round are another step).  A matrix has to lie
+                  on one shard: with several shards use a RangePartitioner
+                  whose blocks hold whole matrices.  M is checkpointed as
+                  the accumulator.
     """
 
     def __init__(self, part: Partitioner, shard: int, dim: int,
