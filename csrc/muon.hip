@@ -109,6 +109,7 @@ struct Momentum {
   const float* grads;
   const int64_t* rows;   // sorted
   const int64_t* order;  // place of the j-th in grads, or null: j
+  const float* sums;     // place n is the first of k_long_runs' sums
   int64_t n;
   float mu;
   bool nesterov;
@@ -123,7 +124,8 @@ __device__ inline int64_t several(int64_t j) { return -2 - j; }
 // push.
 __device__ inline float4 row_gradient(const Momentum& q, int64_t place,
                                       int64_t row, int dim, int c, int held) {
-  float4 g = load_quad(q.grads + place * dim + c, place >= 0 ? held : 0);
+  const float* from = place < q.n ? q.grads : q.sums;
+  float4 g = load_quad(from + place * dim + c, place >= 0 ? held : 0);
   if (place < -1)
     for (int64_t j = several(place); j < q.n && q.rows[j] == row; ++j) {
       const float4 h = load_quad(
@@ -290,9 +292,95 @@ __global__ __launch_bounds__(256) void k_places_any(
   __syncthreads();
   if (t < count)
     place[r0 + t] = named > 1 ? several(first) : named ? only[t] : -1;
-  if (t == 255 && r0 + count == total && run < n) sorted[run] = -1;
+  if (r0 + count == total) {  // the last window: no row from here on
+    if (t == 255) sums[0] = run;
+    __syncthreads();
+    for (int j = sums[0] + t; j < n; j += 256) sorted[j] = -1;
+  }
   if (t == 0 && chunk == 0)
     touched[b] = ends[0][1] | ends[1][1] | ends[2][1] | ends[3][1];
+}
+
+// Rows that a push names more than LONG times (a frequent word of a batch):
+// sums[x] is the sum of the one whose run begins in the x-th LONG places of the
+// sorted push, in the push's order, and the row's place is n + x.  A block
+// takes WIDTH columns: all its threads load, 128 gradients at a time, and a
+// thread a column adds.  Bound by those additions and the latency of a turn's
+// loads: 16 to 30 ns a gradient, where row_gradient, whose loads wait for each
+// other, takes 0.3 to 0.9 us (3952 x 32, 16,000 gradients, half of them of one
+// row: 222 us a step, 2468 without; 2048 x 512, 100,000: 1755, 43483).  A push
+// without such rows pays the launch, 2 us.
+constexpr int LONG = 64;
+
+template <int WIDTH>
+__global__ __launch_bounds__(256) void k_long_runs(
+    float* __restrict__ sums, int64_t* __restrict__ place, Momentum q,
+    int64_t total, int64_t dim) {
+  constexpr int TURN = 128, EACH = TURN * WIDTH / 256;
+  __shared__ float tile[TURN * WIDTH];
+  __shared__ int64_t from[2][TURN];  // places in grads
+  __shared__ int counts[2][TURN / WAVE];
+  __shared__ int64_t first;
+  const int t = threadIdx.x;
+  if (t < LONG) {  // one wave; runs this long begin once in LONG places
+    const int64_t j = (int64_t)blockIdx.x * LONG + t;
+    bool begins = false;
+    if (j + LONG < q.n) {
+      const int64_t r = q.rows[j];
+      begins = r >= 0 && r < total && q.rows[j + LONG] == r &&
+               (j == 0 || q.rows[j - 1] != r);
+    }
+    const uint64_t votes = __ballot(begins);
+    if (t == 0) first = votes ? j + __builtin_ctzll(votes) : -1;
+  }
+  __syncthreads();
+  if (first < 0) return;
+  const int64_t row = q.rows[first];
+  auto look = [&](int64_t j, int buffer) {
+    if (t >= TURN) return;
+    const bool same = j + t < q.n && q.rows[j + t] == row;
+    from[buffer][t] = !same ? -1 : q.order ? q.order[j + t] : j + t;
+    const uint64_t votes = __ballot(same);
+    if (t % WAVE == 0) counts[buffer][t / WAVE] = __popcll(votes);
+  };
+  for (int64_t c0 = (int64_t)blockIdx.y * WIDTH; c0 < dim;
+       c0 += (int64_t)gridDim.y * WIDTH) {
+    float v[EACH], sum = 0.0f;
+    auto fetch = [&](int buffer) {
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int64_t g = from[buffer][(t + e * 256) / WIDTH];
+        const int64_t c = c0 + t % WIDTH;
+        v[e] = g >= 0 && c < dim ? q.grads[g * dim + c] : 0.0f;
+      }
+    };
+    __syncthreads();  // of the columns before
+    look(first, 0);
+    look(first + TURN, 1);
+    __syncthreads();
+    fetch(0);
+    int64_t j = first;
+    for (int buffer = 0;; buffer ^= 1) {
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) tile[t + e * 256] = v[e];
+      const int count = counts[buffer][0] + counts[buffer][1];
+      const bool more = counts[buffer ^ 1][0] != 0;
+      __syncthreads();
+      if (more) {
+        fetch(buffer ^ 1);
+        look(j + 2 * TURN, buffer);
+      }
+      if (t < WIDTH) {
+#pragma unroll 16
+        for (int k = 0; k < count; ++k) sum += tile[k * WIDTH + t];
+      }
+      __syncthreads();
+      if (!more) break;
+      j += TURN;
+    }
+    if (t < WIDTH && c0 + t < dim) sums[blockIdx.x * dim + c0 + t] = sum;
+  }
+  if (blockIdx.y == 0 && t == 0) place[row] = q.n + blockIdx.x;
 }
 
 // active[0] = how many of up to 32768 matrices are touched, then which.
@@ -2167,11 +2255,26 @@ void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
                        order.defined() ? order.data_ptr<int64_t>() : nullptr,
                        n, matrix_rows, windows);
   }
-  const Momentum q{u.data_ptr<float>(),       momentum.data_ptr<float>(),
-                   grads.data_ptr<float>(),   rows.data_ptr<int64_t>(),
-                   order.defined() ? order.data_ptr<int64_t>() : nullptr,
-                   n,                         (float)mu,
-                   nesterov};
+  Momentum q{u.data_ptr<float>(),       momentum.data_ptr<float>(),
+             grads.data_ptr<float>(),   rows.data_ptr<int64_t>(),
+             order.defined() ? order.data_ptr<int64_t>() : nullptr,
+             nullptr,                   n,
+             (float)mu,                 nesterov};
+  at::Tensor sums;
+  if (!sorted_unique && n > LONG) {
+    const int64_t chunks = (n + LONG - 1) / LONG;
+    sums = at::empty({chunks * dim}, table.options());
+    q.sums = (const float*)((uintptr_t)sums.data_ptr<float>() -
+                            (uintptr_t)(n * dim) * sizeof(float));
+    auto go = [&](auto* kfn, int width) {
+      const int64_t slices = std::min<int64_t>((dim + width - 1) / width, 65535);
+      hipLaunchKernelGGL(kfn, dim3(chunks, slices), dim3(256), 0, stream,
+                         sums.data_ptr<float>(), at_, q, total, dim);
+    };
+    if (dim <= 16) go(k_long_runs<16>, 16);
+    else if (dim <= 32) go(k_long_runs<32>, 32);
+    else go(k_long_runs<64>, 64);
+  }
   // one pass makes U and sums G where a block holds a row and a square of G
   const bool fused = is_thin(at::kFloat, batch, matrix_rows, dim) && dim > NARROW &&
                      dim <= SUPER && matrix_rows >= dim && batch <= 32768;
