@@ -2230,9 +2230,10 @@ void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
   const bool captured = capture != hipStreamCaptureStatusNone;
   const bool any = !sorted_unique && n <= SHORT &&
                    (windows <= 1024 || (captured && windows <= 1 << 20));
-  TORCH_CHECK(sorted_unique || any || !captured, "a push of more than ", SHORT,
-              " rows in any order, or into more than ", 1 << 20,
-              " matrices, cannot be captured");
+  TORCH_CHECK(sorted_unique || any || !captured, "a push in any order of "
+              "more than ", SHORT, " rows, or into a table of more than ",
+              1 << 20, " windows (256 rows of a matrix or what is left of "
+              "one), cannot be captured");
   auto touched = at::empty({batch}, table.options().dtype(at::kInt));
   auto u = at::empty_like(table);
   auto place = at::empty({total}, rows.options());

@@ -304,7 +304,9 @@ def apply_muon(table: torch.Tensor, momentum: torch.Tensor,
     outside the table are left out.  Repeated rows are summed in the order
     that they come in.  ``sorted_unique``: the caller guarantees ``rows``
     ascending with no duplicates, so the pre-sort is skipped.  Of other
-    pushes, those of up to 16384 rows can be captured into a graph."""
+    pushes, those of up to 16384 rows can be captured into a graph, for
+    tables of up to 2^20 windows (256 rows of a matrix, or what is left of
+    one)."""
     a, b, c = _check_chain("apply_muon", steps, coeffs, eps)
     if table.dim() != 2 or table.dtype != torch.float32 \
             or momentum.shape != table.shape \
