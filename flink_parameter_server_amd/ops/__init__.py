@@ -284,6 +284,12 @@ def orthogonalize(x: torch.Tensor, steps: int = 5,
     return out.view(x.shape)
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether contiguous tensors share memory."""
+    return a.data_ptr() < b.data_ptr() + b.nbytes \
+        and b.data_ptr() < a.data_ptr() + a.nbytes
+
+
 def apply_muon(table: torch.Tensor, momentum: torch.Tensor,
                rows: torch.Tensor, grads: torch.Tensor, lr: float,
                mu: float = 0.95, nesterov: bool = True,
@@ -317,7 +323,7 @@ def apply_muon(table: torch.Tensor, momentum: torch.Tensor,
                          f"{tuple(momentum.shape)}")
     if not table.is_contiguous() or not momentum.is_contiguous():
         raise ValueError("apply_muon: table and momentum must be contiguous")
-    if table.numel() and table.data_ptr() == momentum.data_ptr():
+    if _overlap(table, momentum):
         raise ValueError("apply_muon: table and momentum are the same memory")
     if rows.dim() != 1 or rows.dtype not in (torch.int64, torch.int32) \
             or grads.dtype != torch.float32 \
@@ -336,6 +342,8 @@ def apply_muon(table: torch.Tensor, momentum: torch.Tensor,
     if not rows.numel() or not table.numel():
         return
     rows, grads = rows.long().contiguous(), grads.detach().contiguous()
+    if _overlap(grads, momentum) or _overlap(grads, table):
+        grads = grads.clone()
     args = (lr, mu, nesterov, weight_decay, int(steps), m)
     if _cuda(table):
         hip.ext().apply_muon(table, momentum, rows, bool(sorted_unique), grads,
