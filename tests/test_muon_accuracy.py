@@ -124,3 +124,42 @@ def test_alone_and_in_a_batch(b, m, n):
         near = float((f32[k].double() - want[k]).norm())
         got = ops.orthogonalize(x[k:k + 1].cuda())[0].cpu()
         assert float((got.double() - want[k]).norm()) <= 8 * near
+
+
+def low_rank(kind, m, n):
+    g = torch.Generator().manual_seed(m + n)
+    if kind == "ones":  # every value is rounded alike
+        return torch.ones(1, m, n) / 3
+    if kind == "column":
+        x = torch.zeros(1, m, n)
+        x[:, :, n // 2] = torch.randn(m, generator=g)
+        return x
+    if kind == "row":
+        x = torch.zeros(1, m, n)
+        x[:, m // 2] = torch.randn(n, generator=g)
+        return x
+    return torch.bmm(torch.randn(1, m, 2, generator=g),
+                     torch.randn(1, 2, n, generator=g))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["ones", "column", "row", "rank2"])
+@pytest.mark.parametrize("m,n", [(40, 60), (6040, 32), (32, 6040), (900, 128),
+                                 (300, 900), (900, 300), (400, 520),
+                                 (520, 400), (1000, 700)])
+def test_low_rank(kind, m, n):
+    """Singular values of zero: the chain multiplies what lies there by
+    a^5 = 485.  P is 485 (1 - v v') + p v v', whose values' sizes are a matrix
+    of norm 970 at most, and |X| is 1.  P U is made of values of P and U that
+    are 2^-24 off, without the product of their lows (2^-24), with three f32
+    additions for 32 of s places and a few at the ends: all of them 970 times
+    2^-24.  Steps on X make as many of them, each multiplied by what follows:
+    no more than five times that."""
+    x = low_rank(kind, m, n)
+    s = min(m, n)
+    limit = 970 * (6 + 3 * (s // 32 + 1)) * 2.0 ** -24
+    if not (s <= 64 or s <= 320 and max(m, n) >= 3 * s):
+        limit *= 5
+    off = float((ops.orthogonalize(x.cuda()).cpu().double()
+                 - exact(x)).norm())
+    assert off <= limit
