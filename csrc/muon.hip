@@ -5,17 +5,25 @@
 //     X = U / (|U|_F + eps),  then `steps` times
 //     G = X X^T (on the side of length s),  X <- (a I + b G + c G^2) X.
 //
-// Two ways to the same result, both f32-exact to a few last places:
+// Two ways to the same result.  Both hold the operands of their large products
+// in two f16 planes, hi + lo, and add in f32: 22 to 24 bits of a value and down
+// to 2^-37 of its matrix's norm, and the product of two lows is left out.  That
+// is three f16 products in place of one f32 product, which costs 16 / 3 as much
+// at this card's matrix rates.  Off the chain in 64 bits by 1e-7 to 4e-6 of the
+// result's norm where singular values are alike (steps in f32: 2e-6 to 4e-6).
+// What lies along a singular value near zero is multiplied by a^steps = 485,
+// roundings too: where all but a few are zero the result is up to 4e-4 off (as
+// steps in f32 are, though not for the same matrices: a 300 x 900 matrix of
+// equal values is 3.5e-4 off on the thin route, 1e-5 in f32; random ones of
+// rank 1 are 1e-4 to 2e-4 off on the wide route, 2e-4 to 4e-4 in f32).
 //
 // thin   G is taken once, in f64 over the long axis; the steps are then taken
 //        on s x s matrices alone (each multiplies X by Q = a I + b G + c G^2
 //        and G by Q^2), and one product applies P = Q_1 ... Q_k to U.  Two
 //        passes over the values instead of two a step.  G has to be f64: an
 //        error in it grows by a^2 = 12 with every step.
-// wide   the chain as written, with every operand held as two f16 planes,
-//        hi + lo (22 bits): a b = hi hi + hi lo + lo hi on the f16 matrix
-//        units, accumulated in f32.  Three f16 products cost 3 / 16 of one
-//        f32 product at this card's matrix rates.
+// wide   the chain as written, with every operand in planes:
+//        a b = hi hi + hi lo + lo hi on the f16 matrix units.
 
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContext.h>
@@ -1710,7 +1718,13 @@ struct Chain {
   const int64_t* place = nullptr;
 };
 
-// Measured, thin against wide.  f32: 1 x 128 x 512 82 us, 98; 1 x 200 x 600
+// Thin touches the values twice and takes some 14 small products in f64, which
+// wait for each other: their time is that of their launches while batch * s is
+// small and that of the f64 units, batch * s^3, above.  Wide takes three
+// products over the values a step, batch * s^2 * long.  So thin is the faster
+// one from a ratio long / s that is small (3) while the products fill few CUs
+// and large (16) where they fill the card; s * s in f64 has to fit its kernels
+// (THIN_MAX).  Measured, thin against wide.  f32: 1 x 128 x 512 82 us, 98; 1 x 200 x 600
 // 104, 118; 1 x 256 x 512 115, 111; 1 x 320 x 1280 137, 162; of many matrices
 // the small products take longer: 4 x 200 x 800 147, 130; 16 x 128 x 1024 158,
 // 141; 8 x 200 x 3200 225, 246; 16 x 128 x 2048 164, 193.  bfloat16, whose wide
@@ -1943,10 +1957,11 @@ void run_product(const Chain& c, Product pr, const Cut& cut, int jobs = 1) {
 // How many steps in a row are taken on the Gram matrix before P is applied to
 // X; 1 for none.  With L = r s a step costs 3 r + 1 products of s^3 on X, and n
 // in a row cost 3 r + 4 n - 3.  What G is off grows by q^2 with every step: n is
-// bounded so that it does so by 200 in all (three of Muon's).  The result of
-// five is then a few parts in 10^5 off, whatever the singular values: far below
-// bfloat16's rounding, but several times what steps on X leave, so the other
-// types take those.
+// bounded so that it does so by 200 in all (three of Muon's).  Before it is
+// rounded the result of five is then 3e-6 (singular values alike) to 2e-4 off
+// (all values equal), where steps on X leave 2e-6 and 1e-5: at most an eighth of
+// bfloat16's rounding, which is 1.7e-3, but too much for the other types.
+// Measured: 8 x 512 x 2048 303 us, on X 424.
 template <typename T>
 int steps_on_gram(const Chain& c, int64_t s, int64_t long_) {
   if (!std::is_same_v<T, __hip_bfloat16> || long_ * 2 < s * 3) return 1;

@@ -197,7 +197,9 @@ def cache_write(cache: torch.Tensor, values: torch.Tensor,
     more; smaller ones have a scale of 2^-126).  A row with an infinity or NaN reads back as
     NaN throughout.  Slots outside the cache are padding and not written.
     Of several rows for one slot the last one is kept; ``unique=True``
-    asserts that there are none (and saves the pass that finds out)."""
+    asserts that there are none and saves the pass that finds out, which
+    takes 4 bytes a record of the cache (64 rows into 10^7 records: 15 us,
+    5 without)."""
     if _cuda(cache):
         hip.ext().cache_write(cache, values, slots, fmt, unique)
         return
@@ -262,8 +264,12 @@ def orthogonalize(x: torch.Tensor, steps: int = 5,
     times X <- a X + (b G + c G^2) X with G = X X^T.  Singular values near
     zero stay there, the others come near one.
 
-    Computed to f32 accuracy whatever the type, rounded once at the end; the
-    result is new and contiguous.  A matrix that holds an infinity or NaN
+    Computed in f32, on the device with products of 22 to 24 bits, whatever
+    the type, and rounded once at the end: before that, off by a few 1e-6 of
+    the result's norm where singular values are alike, and by up to 4e-4
+    where all but a few are near zero, whose roundings the steps multiply.
+    In last places a result may depend on how many matrices there are, not
+    on what the others hold.  The result is new and contiguous.  A matrix that holds an infinity or NaN
     gives NaN throughout, a matrix of zeros gives zeros.  Has no gradient."""
     if x.dim() < 2 or x.dtype not in _VALUE_TYPES:
         raise ValueError("orthogonalize: x must be matrices of float32, "
