@@ -330,65 +330,68 @@ __global__ __launch_bounds__(256) void k_long_runs(
   __shared__ int counts[2][TURN / WAVE];
   __shared__ int64_t first;
   const int t = threadIdx.x;
-  if (t < LONG) {  // one wave; runs this long begin once in LONG places
-    const int64_t j = (int64_t)blockIdx.x * LONG + t;
-    bool begins = false;
-    if (j + LONG < q.n) {
-      const int64_t r = q.rows[j];
-      begins = r >= 0 && r < total && q.rows[j + LONG] == r &&
-               (j == 0 || q.rows[j - 1] != r);
-    }
-    const uint64_t votes = __ballot(begins);
-    if (t == 0) first = votes ? j + __builtin_ctzll(votes) : -1;
-  }
-  __syncthreads();
-  if (first < 0) return;
-  const int64_t row = q.rows[first];
-  auto look = [&](int64_t j, int buffer) {
-    if (t >= TURN) return;
-    const bool same = j + t < q.n && q.rows[j + t] == row;
-    from[buffer][t] = !same ? -1 : q.order ? q.order[j + t] : j + t;
-    const uint64_t votes = __ballot(same);
-    if (t % WAVE == 0) counts[buffer][t / WAVE] = __popcll(votes);
-  };
-  for (int64_t c0 = (int64_t)blockIdx.y * WIDTH; c0 < dim;
-       c0 += (int64_t)gridDim.y * WIDTH) {
-    float v[EACH], sum = 0.0f;
-    auto fetch = [&](int buffer) {
-#pragma unroll
-      for (int e = 0; e < EACH; ++e) {
-        const int64_t g = from[buffer][(t + e * 256) / WIDTH];
-        const int64_t c = c0 + t % WIDTH;
-        v[e] = g >= 0 && c < dim ? q.grads[g * dim + c] : 0.0f;
+  for (int64_t x = blockIdx.x; x * LONG < q.n; x += gridDim.x) {
+    __syncthreads();  // of the run before
+    if (t < LONG) {  // one wave; runs this long begin once in LONG places
+      const int64_t j = x * LONG + t;
+      bool begins = false;
+      if (j + LONG < q.n) {
+        const int64_t r = q.rows[j];
+        begins = r >= 0 && r < total && q.rows[j + LONG] == r &&
+                 (j == 0 || q.rows[j - 1] != r);
       }
-    };
-    __syncthreads();  // of the columns before
-    look(first, 0);
-    look(first + TURN, 1);
+      const uint64_t votes = __ballot(begins);
+      if (t == 0) first = votes ? j + __builtin_ctzll(votes) : -1;
+    }
     __syncthreads();
-    fetch(0);
-    int64_t j = first;
-    for (int buffer = 0;; buffer ^= 1) {
+    if (first < 0) continue;
+    const int64_t row = q.rows[first];
+    auto look = [&](int64_t j, int buffer) {
+      if (t >= TURN) return;
+      const bool same = j + t < q.n && q.rows[j + t] == row;
+      from[buffer][t] = !same ? -1 : q.order ? q.order[j + t] : j + t;
+      const uint64_t votes = __ballot(same);
+      if (t % WAVE == 0) counts[buffer][t / WAVE] = __popcll(votes);
+    };
+    for (int64_t c0 = (int64_t)blockIdx.y * WIDTH; c0 < dim;
+         c0 += (int64_t)gridDim.y * WIDTH) {
+      float v[EACH], sum = 0.0f;
+      auto fetch = [&](int buffer) {
 #pragma unroll
-      for (int e = 0; e < EACH; ++e) tile[t + e * 256] = v[e];
-      const int count = counts[buffer][0] + counts[buffer][1];
-      const bool more = counts[buffer ^ 1][0] != 0;
+        for (int e = 0; e < EACH; ++e) {
+          const int64_t g = from[buffer][(t + e * 256) / WIDTH];
+          const int64_t c = c0 + t % WIDTH;
+          v[e] = g >= 0 && c < dim ? q.grads[g * dim + c] : 0.0f;
+        }
+      };
+      __syncthreads();  // of the columns before
+      look(first, 0);
+      look(first + TURN, 1);
       __syncthreads();
-      if (more) {
-        fetch(buffer ^ 1);
-        look(j + 2 * TURN, buffer);
-      }
-      if (t < WIDTH) {
+      fetch(0);
+      int64_t j = first;
+      for (int buffer = 0;; buffer ^= 1) {
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) tile[t + e * 256] = v[e];
+        const int count = counts[buffer][0] + counts[buffer][1];
+        const bool more = counts[buffer ^ 1][0] != 0;
+        __syncthreads();
+        if (more) {
+          fetch(buffer ^ 1);
+          look(j + 2 * TURN, buffer);
+        }
+        if (t < WIDTH) {
 #pragma unroll 16
-        for (int k = 0; k < count; ++k) sum += tile[k * WIDTH + t];
+          for (int k = 0; k < count; ++k) sum += tile[k * WIDTH + t];
+        }
+        __syncthreads();
+        if (!more) break;
+        j += TURN;
       }
-      __syncthreads();
-      if (!more) break;
-      j += TURN;
+      if (t < WIDTH && c0 + t < dim) sums[x * dim + c0 + t] = sum;
     }
-    if (t < WIDTH && c0 + t < dim) sums[blockIdx.x * dim + c0 + t] = sum;
+    if (blockIdx.y == 0 && t == 0) place[row] = q.n + x;
   }
-  if (blockIdx.y == 0 && t == 0) place[row] = q.n + blockIdx.x;
 }
 
 // active[0] = how many of up to 32768 matrices are touched, then which.
@@ -2283,8 +2286,9 @@ void apply_muon(at::Tensor table, at::Tensor momentum, at::Tensor rows,
     q.sums = (const float*)((uintptr_t)sums.data_ptr<float>() -
                             (uintptr_t)(n * dim) * sizeof(float));
     auto go = [&](auto* kfn, int width) {
-      const int64_t slices = std::min<int64_t>((dim + width - 1) / width, 65535);
-      hipLaunchKernelGGL(kfn, dim3(chunks, slices), dim3(256), 0, stream,
+      const dim3 grid(std::min<int64_t>(chunks, 1 << 20),
+                      std::min<int64_t>((dim + width - 1) / width, 65535));
+      hipLaunchKernelGGL(kfn, grid, dim3(256), 0, stream,
                          sums.data_ptr<float>(), at_, q, total, dim);
     };
     if (dim <= 16) go(k_long_runs<16>, 16);

@@ -95,6 +95,17 @@ def test_replayed_with_other_repeats():
 
 
 @pytest.mark.gpu
+def test_more_gradients_than_a_launch_has_blocks_for():
+    """2^26 places are a launch's; ones are summed exactly below 2^24."""
+    R, pushed = 700, 2 ** 26 + 12345
+    rows = torch.randint(0, R - 1, (pushed,), device="cuda")
+    rows[::7] = R - 1  # the last of the sorted ones: 9.6 million
+    table, mo = (torch.zeros(R, 1, device="cuda") for _ in range(2))
+    ops.apply_muon(table, mo, rows, torch.ones(pushed, 1, device="cuda"), 0.1)
+    assert torch.equal(mo.view(-1).long(), torch.bincount(rows, minlength=R))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("R,n", [(3952, 32), (20000, 100), (2048, 512)])
 def test_one_row_does_not_hold_up_a_step(R, n):
     """100,000 gradients of one row: a pass over them and a sort take a
