@@ -16,7 +16,6 @@ from typing import List, Optional, Tuple
 import torch
 
 from . import ops
-from .api import ServerLogic
 from .parallel.partitioner import Partitioner
 
 
@@ -191,7 +190,7 @@ class ShardedTable:
                                                  self.data.dtype))
 
 
-class TableServerLogic(ServerLogic):
+class TableServerLogic:
     """ServerLogic over a ShardedTable — the production default server.
 
     Semantics parity: ``SimplePSLogic(paramInit, paramUpdate)`` with
@@ -240,7 +239,8 @@ class TableServerLogic(ServerLogic):
         as there are workers, however small their shares of the gradient
         are."""
         if len(pushes) == 1 or not self.whole_steps:
-            super().on_pushes_recv(pushes, ps)
+            for ids, deltas in pushes:
+                self.on_push_recv(ids, deltas, ps)
             return
         self._joined = True
         try:
