@@ -238,6 +238,10 @@ def _check_chain(name: str, steps: int, coeffs: Sequence[float],
     if not _bounded(a, b, c, int(steps)):
         raise ValueError(f"{name}: with coeffs {coeffs!r} singular values "
                          f"grow beyond 3.9 in {steps} steps")
+    if abs(a) ** int(steps) < 2.0 ** -12:
+        raise ValueError(f"{name}: with coeffs {coeffs!r} singular values "
+                         f"near zero shrink to less than 2^-12 of what they "
+                         f"were in {steps} steps")
     return a, b, c
 
 
